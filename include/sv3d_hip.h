@@ -8,7 +8,9 @@
  *
  * Conventions
  *   - All pointers are DEVICE pointers to contiguous row-major fp32 / int32
- *     buffers owned by the caller and borrowed for the call.
+ *     buffers owned by the caller and borrowed for the call (the layer norm and
+ *     optimizer calls at the end name further types; parameter structs and their
+ *     arrays are host memory).
  *   - `stream` is a hipStream_t passed as void*; every call only enqueues work
  *     on it (no allocation, no host synchronisation), so calls are graph-capture
  *     safe and re-entrant: the library keeps no mutable state between calls (the one
@@ -328,6 +330,93 @@ int sv3d_distance_transform(const float *masks, int32_t B, int32_t H, int32_t W,
 #define SV3D_DT_STATIC_MAX_PIXELS (4 * 1024 * 1024)   /* e.g. 64 masks of 256 x 256 */
 int sv3d_distance_transform_static(const float *masks, int32_t B, int32_t H, int32_t W,
                                    int32_t barrier, float k, float *out, void *stream);
+
+/* ---- the training step around the networks' matrix products -------------------------------------
+ * Layer norm (the transformer camera head of the reference's network, mesh_net.py:468-536) and the
+ * optimizer step over all weights (train_utils.py:165-172,201-214: unscale, clip_grad_norm_, Adam).
+ * Element types of these calls: */
+enum { SV3D_F32 = 0, SV3D_F16 = 1, SV3D_BF16 = 2 };
+
+/* y = (x - mean) * rstd * weight + bias over each row of `cols` elements, mean and
+ * rstd = 1/sqrt(var + eps) being the row's own (var divides by cols).  Statistics and arithmetic in fp32. */
+typedef struct sv3d_layer_norm_params {
+    int64_t rows, cols;    /* rows may be 0                                                      */
+    int64_t x_stride;      /* elements from one row of x to the next; 0 repeats one row          */
+    int64_t dy_stride;     /* the same for dy (backward only)                                    */
+    int32_t x_type;        /* of x and dx                                                        */
+    int32_t y_type;        /* of y and dy: x_type, or SV3D_F32                                   */
+    int32_t param_type;    /* of weight, bias and their gradients: x_type, or SV3D_F32           */
+    float eps;
+} sv3d_layer_norm_params;
+
+/* `weight`, `bias` may be NULL (1 and 0), `mean`, `rstd` [rows] too (nobody will call the backward).
+ * y is contiguous. */
+int sv3d_layer_norm_forward(const sv3d_layer_norm_params *p, const void *x, const void *weight, const void *bias,
+                            void *y, float *mean, float *rstd, void *stream);
+
+/* Gradients of the call above; each of dx (contiguous), dweight, dbias may be NULL.  dweight and dbias
+ * are sums over the rows in an order that the sizes fix; they need `workspace`, at least
+ * sv3d_layer_norm_workspace() bytes, 16-byte aligned, whose content does not matter. */
+int sv3d_layer_norm_workspace(const sv3d_layer_norm_params *p, size_t *bytes);
+int sv3d_layer_norm_backward(const sv3d_layer_norm_params *p, const void *x, const void *dy, const void *weight,
+                             const float *mean, const float *rstd, void *dx, void *dweight, void *dbias,
+                             void *workspace, size_t workspace_bytes, void *stream);
+
+/* One tensor of an optimizer step.  With `state_bits` 32, exp_avg and exp_avg_sq are fp32 [numel] and
+ * `scales` is NULL.  With 8 they are bytes [numel] and `scales` is bytes [ceil(numel/128)][2]:
+ * blocks of SV3D_STATE_BLOCK consecutive elements share a power of two for each moment, held as a
+ * byte (exp_avg's, exp_avg_sq's).  A code c of exp_avg with byte e stands for
+ *   (-1)^(c>>7) * (E ? (1 + M/8) 2^(E-7) : M/8 2^-6) * 2^(e-134),   E = c>>3 & 15, M = c & 7, 0x7f / 0xff NaN,
+ * one of exp_avg_sq for
+ *   (E ? (1 + M/8) 2^(E-15) : M/8 2^-14) * 2^(e-142),               E = c>>3, M = c & 7, 0xff NaN.
+ * Bytes below 20 (exp_avg) and 34 (exp_avg_sq) count as these: all zeros is a fresh state. */
+enum { SV3D_STATE_BLOCK = 128 };
+typedef struct sv3d_adamw_tensor {
+    void *param;
+    const void *grad;      /* of the weight's type                                               */
+    void *exp_avg;
+    void *exp_avg_sq;
+    uint8_t *scales;
+    float *step;           /* number of steps this tensor has taken: read, then one is added     */
+    int64_t numel;         /* may be 0                                                           */
+    int32_t type;          /* SV3D_F32, SV3D_F16 or SV3D_BF16                                    */
+    int32_t state_bits;    /* 32 or 8                                                            */
+} sv3d_adamw_tensor;
+
+/* Sums of squares of the gradients (grad, numel and type of each entry are read), in double:
+ * sv3d_grad_square_sums_count() numbers whose sum is the squared norm of all of them together. */
+int sv3d_grad_square_sums_count(const sv3d_adamw_tensor *tensors, int32_t num_tensors, int32_t *count);
+int sv3d_grad_square_sums(const sv3d_adamw_tensor *tensors, int32_t num_tensors, double *sums, int32_t count,
+                          void *stream);
+
+/* With S = *grad_scale (1 if NULL), G = sqrt(sum of square_sums) / S and
+ *   g  = grad / S * min(1, max_norm / (G + 1e-6))       (no factor if square_sums is NULL)
+ *   t  = step + 1;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   param = param (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * in fp32; the weight is rounded to its type to nearest, 8-bit moments are rounded up or down with the
+ * probability of what is cut off, decided by a hash of (element, t, seed), and a positive exp_avg_sq
+ * never becomes zero.  `maximize` negates g.  If *found_inf is not 0 nothing is changed.  lr is read from
+ * `lr_device` where that is not NULL.  *total_norm (may be NULL) receives G.
+ * `workspace`: sv3d_adamw_workspace() bytes, 16-byte aligned; its content does not matter. */
+typedef struct sv3d_adamw_params {
+    double lr, beta1, beta2, eps, weight_decay, max_norm;
+    const float *lr_device;
+    const float *grad_scale;
+    const float *found_inf;
+    const double *square_sums;
+    float *total_norm;
+    int32_t num_square_sums;
+    int32_t maximize;
+    uint32_t seed;
+} sv3d_adamw_params;
+
+int sv3d_adamw_workspace(int32_t num_tensors, size_t *bytes);
+int sv3d_adamw_step(const sv3d_adamw_params *p, const sv3d_adamw_tensor *tensors, int32_t num_tensors,
+                    void *workspace, size_t workspace_bytes, void *stream);
+
+/* The values that 8-bit moments stand for, as bf16 (which holds every one of them exactly). */
+int sv3d_moment_values(const uint8_t *exp_avg, const uint8_t *exp_avg_sq, const uint8_t *scales, int64_t numel,
+                       void *exp_avg_out, void *exp_avg_sq_out, void *stream);
 
 #ifdef __cplusplus
 }

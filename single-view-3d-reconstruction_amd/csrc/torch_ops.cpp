@@ -20,33 +20,11 @@
 // There is no CPU kernel: CPU tensors fail in the dispatcher.  Inputs of other floating types
 // (autocast regions hand over fp16) are computed in fp32 and gradients are returned in the
 // inputs' types.  torch is used for device memory, streams and autograd plumbing only.
-#include <ATen/ATen.h>
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <torch/autograd.h>
-#include <torch/library.h>
-
-#include <string>
-#include <tuple>
-#include <utility>
-#include <vector>
-
-#include "sv3d_hip.h"
+#include "torch_util.h"
 
 namespace {
 
-using at::Tensor;
-using c10::optional;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-using IntList = at::IntArrayRef;
 using FloatList = at::ArrayRef<double>;
-
-// ---- small helpers ---------------------------------------------------------------------------
-void check_status(int st, const char *what)
-{
-    TORCH_CHECK(st == SV3D_OK, what, " failed: ", sv3d_strerror(st), " (status ", st, ")");
-}
 
 // fp32 contiguous form of a tensor: the tensor itself when it already is that (these kernels run
 // below autograd, nothing they do is recorded), a converted copy otherwise
@@ -56,24 +34,9 @@ Tensor f32c(const Tensor &t)
     return t.to(at::kFloat).contiguous();
 }
 
-struct Launch {
-    c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard;
-    void *stream;
-    explicit Launch(const Tensor &t) : guard(t.device())
-    {
-        stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
-    }
-};
-
 const float *fptr(const optional<Tensor> &t) { return t.has_value() && t->defined() && t->numel() > 0 ? t->data_ptr<float>() : nullptr; }
 const float *fptr(const Tensor &t) { return t.defined() && t.numel() > 0 ? t.data_ptr<float>() : nullptr; }
 float *fptr_mut(Tensor &t) { return t.defined() && t.numel() > 0 ? t.data_ptr<float>() : nullptr; }
-
-void same_device(const Tensor &ref, const Tensor &t, const char *name)
-{
-    // a tensor on the host or on another GPU would reach the kernels as a foreign pointer
-    TORCH_CHECK(t.device() == ref.device(), name, " is on ", t.device(), ", expected ", ref.device());
-}
 
 // icfg: raster_size, aa, texture_mode, texture_res, double_side, alpha_only[, backward_enumeration]
 // fcfg: background r g b, near, far, eps, sigma, dist_eps, gamma
@@ -751,12 +714,6 @@ Tensor distance_transform_meta(const Tensor &masks, bool, double)
 }
 
 // ---- dispatcher handles (calls from the autograd kernels go below autograd) ----------------------
-template <class Sig>
-c10::TypedOperatorHandle<Sig> find_op(const char *name)
-{
-    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
-}
-
 using RasterOut = std::tuple<Tensor, Tensor, Tensor>;
 
 RasterOut call_soft_rasterize(const Tensor &fv, const optional<Tensor> &tex, IntList icfg, FloatList fcfg)
@@ -792,8 +749,6 @@ RasterOut call_render_backward(const Tensor &g, const Tensor &v, const Tensor &c
                                        FloatList, bool)>("sv3d::render_backward");
     return op.call(g, v, c, f, tex, rec, saved, mesh_cfg, icfg, fcfg, need_tex);
 }
-
-Tensor cast_like(const Tensor &g, at::ScalarType t) { return g.scalar_type() == t ? g : g.to(t); }
 
 // ---- autograd kernels -----------------------------------------------------------------------------
 struct SoftRasterizeFn : public torch::autograd::Function<SoftRasterizeFn> {

@@ -24,6 +24,9 @@ EXPORTS = (
     "sv3d_laplacian_loss", "sv3d_flatten_loss", "sv3d_mesh_spmv",
     "sv3d_texture_sample", "sv3d_texture_sample_backward", "sv3d_distance_transform",
     "sv3d_distance_transform_workspace", "sv3d_distance_transform_static",
+    "sv3d_layer_norm_forward", "sv3d_layer_norm_workspace", "sv3d_layer_norm_backward",
+    "sv3d_grad_square_sums_count", "sv3d_grad_square_sums", "sv3d_adamw_workspace", "sv3d_adamw_step",
+    "sv3d_moment_values",
 )
 
 
@@ -47,6 +50,35 @@ class MeshInput(ctypes.Structure):
         ("vertices", ctypes.c_void_p), ("cams", ctypes.c_void_p), ("faces", ctypes.c_void_p),
         ("num_vertices", ctypes.c_int32), ("faces_batch", ctypes.c_int32),
         ("offset_z", ctypes.c_float), ("scale", ctypes.c_float * 3), ("shift", ctypes.c_float * 3),
+    ]
+
+
+SV3D_F32, SV3D_F16, SV3D_BF16 = 0, 1, 2
+
+
+class LayerNormParams(ctypes.Structure):
+    """Mirror of `sv3d_layer_norm_params`."""
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("dy_stride", ctypes.c_int64),
+        ("x_type", ctypes.c_int32), ("y_type", ctypes.c_int32), ("param_type", ctypes.c_int32), ("eps", ctypes.c_float),
+    ]
+
+
+class AdamWTensor(ctypes.Structure):
+    """Mirror of `sv3d_adamw_tensor`."""
+    _fields_ = [
+        ("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("exp_avg", ctypes.c_void_p),
+        ("exp_avg_sq", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("step", ctypes.c_void_p),
+        ("numel", ctypes.c_int64), ("type", ctypes.c_int32), ("state_bits", ctypes.c_int32),
+    ]
+
+
+class AdamWParams(ctypes.Structure):
+    """Mirror of `sv3d_adamw_params`."""
+    _fields_ = [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "max_norm")] + [
+        ("lr_device", ctypes.c_void_p), ("grad_scale", ctypes.c_void_p), ("found_inf", ctypes.c_void_p),
+        ("square_sums", ctypes.c_void_p), ("total_norm", ctypes.c_void_p), ("num_square_sums", ctypes.c_int32),
+        ("maximize", ctypes.c_int32), ("seed", ctypes.c_uint32),
     ]
 
 
@@ -95,6 +127,15 @@ def lib():
         L.sv3d_distance_transform.argtypes = [vp, i32, i32, i32, i32, ctypes.c_float, vp, vp, ctypes.c_size_t, vp]
         L.sv3d_distance_transform_workspace.argtypes = [i32, i32, i32, ctypes.POINTER(ctypes.c_size_t)]
         L.sv3d_distance_transform_static.argtypes = [vp, i32, i32, i32, i32, ctypes.c_float, vp, vp]
+        lp, at, i64 = ctypes.POINTER(LayerNormParams), ctypes.POINTER(AdamWTensor), ctypes.c_int64
+        L.sv3d_layer_norm_forward.argtypes = [lp, vp, vp, vp, vp, vp, vp, vp]
+        L.sv3d_layer_norm_workspace.argtypes = [lp, ctypes.POINTER(sz)]
+        L.sv3d_layer_norm_backward.argtypes = [lp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        L.sv3d_grad_square_sums_count.argtypes = [at, i32, ctypes.POINTER(i32)]
+        L.sv3d_grad_square_sums.argtypes = [at, i32, vp, i32, vp]
+        L.sv3d_adamw_workspace.argtypes = [i32, ctypes.POINTER(sz)]
+        L.sv3d_adamw_step.argtypes = [ctypes.POINTER(AdamWParams), at, i32, vp, sz, vp]
+        L.sv3d_moment_values.argtypes = [vp, vp, vp, i64, vp, vp, vp]
         mp = ctypes.POINTER(MeshInput)
         L.sv3d_project_gather.argtypes = [mp, i32, i32, vp, vp]
         L.sv3d_project_scatter.argtypes = [mp, i32, i32, vp, vp, vp, vp]

@@ -1,0 +1,36 @@
+"""Layer norm on the device: entry point of the operators `sv3d::layer_norm` / `sv3d::layer_norm_backward`
+(csrc/torch_train_ops.cpp over the functions of the same names in include/sv3d_hip.h), and the module over it.
+The transformer camera head of the reference's network (nnutils/mesh_net.py:468-536) is made of blocks that each
+end in one.  GPU tensors only.
+"""
+import torch
+
+from .ops import _ops
+
+
+def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
+    """`torch.nn.functional.layer_norm`: normalises over the last `len(normalized_shape)` dimensions of `x`
+    (float32, float16 or bfloat16; any strides, without a copy where rows are contiguous and evenly spaced), then
+    scales and shifts by `weight` and `bias` (of x's type or float32).  Statistics, arithmetic and the sums of the
+    weights' gradients are float32; the result has x's type, under autocast float32 (as torch's).  Differentiable
+    once in x, weight and bias."""
+    shape = [normalized_shape] if isinstance(normalized_shape, int) else list(normalized_shape)
+    need = torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                        or (bias is not None and bias.requires_grad))
+    return _ops.layer_norm(x, shape, weight, bias, eps, torch.is_autocast_enabled("cuda"), need)[0]
+
+
+class LayerNorm(torch.nn.LayerNorm):
+    """`torch.nn.LayerNorm` on the kernel: same arguments, parameters and state dict."""
+
+    def forward(self, x):
+        return layer_norm(x, self.normalized_shape, self.weight, self.bias, self.eps)
+
+
+def convert_layer_norm(module):
+    """Turns every `torch.nn.LayerNorm` inside `module` (or `module` itself) into this `LayerNorm`, in place:
+    parameters, hooks and state dict stay.  Subclasses are left alone.  Returns the number of layers changed."""
+    found = [m for m in module.modules() if type(m) is torch.nn.LayerNorm]
+    for m in found:
+        m.__class__ = LayerNorm
+    return len(found)
