@@ -12,6 +12,7 @@ renderer / Chamfer call pattern of one training iteration:
   Laplacian + flatten regularisers                                       (main.py:515-516)
   barrier distance maps of the masks + texture-flow loss on them         (main.py:259-265,506)
   autocast + GradScaler + clip 0.1 + Adam x2 via nnutils.train_utils.Trainer
+  (--optim adamw / adamw8: the fused step; --fc_norm layer: layer norms in the code layers)
 
 The network is a ResNet-18-shaped encoder re-declared in plain torch with random weights
 (torchvision and pretrained weights are unavailable offline); LPIPS is replaced by an L1
@@ -33,6 +34,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 import soft_renderer as sr
+import sv3d
 from nnutils import geom_utils, loss_utils, train_utils
 from nnutils.softras import SoftNeuralRenderer
 from sv3d import meshgen
@@ -59,9 +61,10 @@ class BasicBlock(nn.Module):
 class Encoder(nn.Module):
     """ResNet-18 trunk -> 200-d code (mesh_net.py:155-208 in shape).  `width` is the channel count
     of the first stage (64 in ResNet-18: 11 M parameters; 8 gives 0.2 M, for rehearsals whose
-    gradients travel through the host)."""
+    gradients travel through the host).  `fc_norm` is what follows the code's linear layers: "batch", as in
+    ResNet-shaped heads, or "layer", whose result does not depend on what else is in the batch or on other ranks."""
 
-    def __init__(self, nz=200, width=64):
+    def __init__(self, nz=200, width=64, fc_norm="batch"):
         super().__init__()
         w = width
         self.stem = nn.Sequential(nn.Conv2d(3, w, 7, 2, 3, bias=False), nn.BatchNorm2d(w), nn.ReLU(True),
@@ -72,8 +75,9 @@ class Encoder(nn.Module):
             cin = cout
         self.layers = nn.Sequential(*layers)
         self.squeeze = nn.Sequential(nn.Conv2d(8 * w, 4 * w, 4, 2, 1), nn.BatchNorm2d(4 * w), nn.LeakyReLU(0.2, True))
-        self.fc = nn.Sequential(nn.Linear(4 * w * 4 * 4, nz), nn.BatchNorm1d(nz), nn.LeakyReLU(0.2, True),
-                                nn.Linear(nz, nz), nn.BatchNorm1d(nz), nn.LeakyReLU(0.2, True))
+        norm = {"batch": nn.BatchNorm1d, "layer": sv3d.LayerNorm}[fc_norm]
+        self.fc = nn.Sequential(nn.Linear(4 * w * 4 * 4, nz), norm(nz), nn.LeakyReLU(0.2, True),
+                                nn.Linear(nz, nz), norm(nz), nn.LeakyReLU(0.2, True))
 
     def forward(self, img):
         x = self.squeeze(self.layers(self.stem(img)))
@@ -82,12 +86,12 @@ class Encoder(nn.Module):
 
 
 class MeshNetLite(nn.Module):
-    def __init__(self, verts, faces, num_cams=8, tex_size=6, nz=200, enc_width=64):
+    def __init__(self, verts, faces, num_cams=8, tex_size=6, nz=200, enc_width=64, fc_norm="batch"):
         super().__init__()
         self.num_cams, self.tex_size = num_cams, tex_size
         self.register_buffer("mean_v", verts)
         self.register_buffer("faces", faces)
-        self.encoder = Encoder(nz, enc_width)
+        self.encoder = Encoder(nz, enc_width, fc_norm)
         self.shape = nn.Linear(nz, verts.shape[0] * 3)
         nn.init.normal_(self.shape.weight, std=1e-4)
         self.cam = nn.Linear(nz, num_cams * 7)
@@ -231,7 +235,8 @@ class ShapeTrainer(train_utils.Trainer):
         o = self.opts
         verts, faces = meshgen.icosphere(o.subdivide)
         verts, faces = torch.from_numpy(verts), torch.from_numpy(faces)
-        self.model = MeshNetLite(verts, faces.long(), o.num_hypo_cams, o.tex_size, enc_width=o.enc_width)
+        self.model = MeshNetLite(verts, faces.long(), o.num_hypo_cams, o.tex_size, enc_width=o.enc_width,
+                                 fc_norm=o.fc_norm)
         if o.channels_last:
             self.model = self.model.to(memory_format=torch.channels_last)
         self.part_basis_generator = PartBasisGenerator(verts.shape[0], o.num_parts)
@@ -327,6 +332,8 @@ def parse(argv=None):
     p.add_argument('--tex_size', type=int, default=6)
     p.add_argument('--enc_width', type=int, default=64,
                    help="channels of the encoder's first stage (64 = ResNet-18; smaller for rehearsals)")
+    p.add_argument('--fc_norm', choices=['batch', 'layer'], default='batch',
+                   help="normalisation of the image code's linear layers; layer: sv3d.LayerNorm")
     p.add_argument('--num_hypo_cams', type=int, default=8)
     p.add_argument('--num_parts', type=int, default=8)
     p.add_argument('--chamf_loss_wt', type=float, default=1.0)

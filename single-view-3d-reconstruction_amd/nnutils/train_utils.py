@@ -38,6 +38,10 @@ main.py:299-308: pose / shape warm-up, alternating vertex updates) names what it
 `--fused_adam 1` (default on a GPU): the reference's `torch.optim.Adam(lr, betas=(beta1, 0.999))`
 (:165-172) with `fused=True` -- the same update rule in one multi-tensor kernel per optimizer
 instead of a dozen, and no host read of the inf check in `GradScaler.step`.
+
+`--optim adamw` / `adamw8`: `sv3d.optim.AdamW`, which takes unscaling and clipping into the step (the gradients are
+read twice and never written) and with `adamw8` holds the moments in 8 bits; with `--weight_decay 0`, the default, its
+update is Adam's.  `--hip_layer_norm 1` turns the `torch.nn.LayerNorm` modules of the networks into `sv3d.LayerNorm`.
 """
 import argparse
 import gc
@@ -79,9 +83,16 @@ def add_training_flags(parser=None):
                    help='1: after a few eager steps, capture forward + loss + backward of a step in a HIP graph '
                         'and replay it (single process, constant batch shape; the optimizer steps stay eager); '
                         '2: capture unscale, clipping, the Adam steps and the scaler update as well '
-                        '(needs --fused_adam 1)')
+                        '(needs --fused_adam 1 or --optim adamw / adamw8)')
     p.add_argument('--fused_adam', type=int, default=1,
                    help="on a GPU, Adam with fused=True: the reference's update rule in one kernel per optimizer")
+    p.add_argument('--optim', choices=['adam', 'adamw', 'adamw8'], default='adam',
+                   help="adam: torch's; adamw: the fused unscale + clip + AdamW step on the GPU; adamw8: the same with "
+                        'moments in 8 bits')
+    p.add_argument('--weight_decay', type=float, default=0.0, help='decoupled weight decay of --optim adamw and adamw8')
+    p.add_argument('--hip_layer_norm', type=int, default=0,
+                   help='1: layer norms of the networks run on the GPU kernel of this package (torch.nn.LayerNorm modules '
+                        'are converted in place)')
     return p
 
 
@@ -233,6 +244,18 @@ class Trainer(object):
         self.init_dataset()
         self.define_model()
         self.define_criterion()
+        optim = getattr(opts, 'optim', 'adam')
+        if optim not in ('adam', 'adamw', 'adamw8'):
+            raise ValueError("unknown --optim %r" % (optim,))
+        if optim != 'adam' and opts.use_sgd:
+            raise ValueError('--optim %s and --use_sgd exclude each other' % optim)
+        if self.device.type != 'cuda' and (optim != 'adam' or getattr(opts, 'hip_layer_norm', 0)):
+            raise RuntimeError('--optim adamw / adamw8 and --hip_layer_norm need a GPU: there is no fallback path')
+        if getattr(opts, 'hip_layer_norm', 0):
+            from sv3d import convert_layer_norm
+            convert_layer_norm(self.model)
+            if self._second_optimizer():
+                convert_layer_norm(self.part_basis_generator)
         self.model = self._wrap(self.model)
         if self._second_optimizer():
             self.part_basis_generator = self._wrap(self.part_basis_generator)
@@ -240,6 +263,11 @@ class Trainer(object):
         def make(params):
             if opts.use_sgd:
                 return torch.optim.SGD(params, lr=opts.learning_rate, momentum=opts.beta1)
+            if optim != 'adam':
+                from sv3d.optim import AdamW
+                return AdamW(params, lr=opts.learning_rate, betas=(opts.beta1, 0.999),
+                             weight_decay=getattr(opts, 'weight_decay', 0.0), max_norm=getattr(opts, 'grad_clip', 0.1),
+                             state_bits=8 if optim == 'adamw8' else 32, seed=getattr(opts, 'seed', 0))
             fused = self.device.type == 'cuda' and bool(getattr(opts, 'fused_adam', 1))
             return torch.optim.Adam(params, lr=opts.learning_rate, betas=(opts.beta1, 0.999),
                                     **({'fused': True} if fused else {}))
@@ -292,16 +320,22 @@ class Trainer(object):
 
     def _optimizer_steps(self, scaler):
         """unscale -> clip_grad_norm_ -> step for each optimizer, then the scaler update
-        (train_utils.py:201-214)."""
+        (train_utils.py:201-214).  The fused step unscales and clips by itself."""
         clip = getattr(self.opts, 'grad_clip', 0.1)
-        scaler.unscale_(self.optimizer)
-        torch.nn.utils.clip_grad_norm_(self.model.parameters(), clip)
-        scaler.step(self.optimizer)
+        pairs = [(self.optimizer, self.model)]
         if self._second_optimizer():
-            scaler.unscale_(self.optimizer_2)
-            torch.nn.utils.clip_grad_norm_(self.part_basis_generator.parameters(), clip)
-            scaler.step(self.optimizer_2)
+            pairs.append((self.optimizer_2, self.part_basis_generator))
+        for optimizer, module in pairs:
+            if not self._fused_step(optimizer):
+                scaler.unscale_(optimizer)
+                torch.nn.utils.clip_grad_norm_(module.parameters(), clip)
+            scaler.step(optimizer)
         scaler.update()
+
+    @staticmethod
+    def _fused_step(optimizer):
+        """Whether it is `sv3d.optim.AdamW` (the package is only imported where it is used)."""
+        return type(optimizer).__module__ == 'sv3d.optim'
 
     def _graph_wanted(self):
         return int(getattr(self.opts, 'cuda_graph', 0)) > 0 and self.device.type == 'cuda' \
@@ -331,9 +365,11 @@ class Trainer(object):
         as a tensor: Adam with fused=True does both once its groups are marked capturable."""
         opts = [self.optimizer] + ([self.optimizer_2] if self._second_optimizer() else [])
         for opt in opts:
+            if self._fused_step(opt):           # counts and the inf check are on the device already
+                continue
             if not isinstance(opt, torch.optim.Adam) or not all(g.get('fused') for g in opt.param_groups):
                 raise RuntimeError('--cuda_graph 2 captures the optimizer steps and needs Adam with --fused_adam 1 '
-                                   '(not --use_sgd); use --cuda_graph 1 to keep the optimizer steps eager')
+                                   'or --optim adamw / adamw8 (not --use_sgd); use --cuda_graph 1 to keep the optimizer steps eager')
             for g in opt.param_groups:
                 g['capturable'] = True
 

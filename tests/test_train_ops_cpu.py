@@ -270,3 +270,24 @@ def test_abi_square_sums_and_moment_values_refuse():
     count = ctypes.c_size_t()
     assert lib.sv3d_adamw_workspace(-1, ctypes.byref(count)) == INVALID
     assert lib.sv3d_adamw_step(ctypes.byref(L.AdamWParams(beta1=0.9, beta2=0.9)), None, 0, None, 0, None) == 0
+
+
+# ---- the trainer ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("argv, error", [(["--optim", "adamw"], RuntimeError), (["--optim", "adamw8"], RuntimeError),
+                                         (["--hip_layer_norm", "1"], RuntimeError), (["--optim", "adamw", "--use_sgd"], ValueError)])
+def test_trainer_on_the_host_refuses_what_needs_a_gpu(tmp_path, argv, error):
+    from nnutils import train_utils
+
+    class T(train_utils.Trainer):
+        def init_dataset(self):
+            self.dataloader = []
+
+        def define_model(self):
+            self.model = torch.nn.Linear(2, 2)
+
+        def define_criterion(self):
+            pass
+
+    o = train_utils.add_training_flags().parse_args(["--checkpoint_dir", str(tmp_path), *argv])
+    with pytest.raises(error):
+        T(o, env=train_utils.DistEnv()).init_training()
