@@ -17,6 +17,85 @@ __device__ inline float to_float(T v) { return (float)v; }
 template <class T>
 __device__ inline T from_float(float v) { return (T)v; }
 
+// N consecutive elements, loaded and stored at once from any address that is a multiple of the element's size (global
+// memory takes wide accesses at any alignment; rows of odd length start anywhere)
+template <class T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Pack {
+    T v[N];
+};
+
+// The same elements as the 32-bit words that they fill, for values that wait in registers: two of 16 bits in each, where a
+// Pack that is put together from single elements would take a register for every one of them.
+template <class T, int N>
+struct Words {
+    static constexpr int kCount = N * (int)sizeof(T) / 4;
+    uint32_t w[kCount];
+    __device__ inline float operator[](int i) const
+    {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        const uint32_t h = w[i / 2];
+        if constexpr (__is_same(T, bf16)) return __uint_as_float(i & 1 ? h & 0xffff0000u : h << 16);
+        return (float)__builtin_bit_cast(f16, (uint16_t)(i & 1 ? h >> 16 : h & 0xffffu));
+    }
+};
+
+// `n` of the elements exist (n <= 0: none), the others are zero
+template <class T, int N>
+__device__ inline Words<T, N> load_words(const T *p, int n)
+{
+    Words<T, N> r;
+    if (n >= N) {
+        const auto q = *reinterpret_cast<const Pack<T, N> *>(p);
+        __builtin_memcpy(r.w, q.v, sizeof(r.w));
+        return r;
+    }
+#pragma unroll
+    for (int i = 0; i < r.kCount; ++i) r.w[i] = 0u;
+    if (n <= 0) return r;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        if (j >= n) break;
+        if constexpr (sizeof(T) == 4)
+            r.w[j] = reinterpret_cast<const uint32_t *>(p)[j];
+        else
+            r.w[j / 2] |= (uint32_t) reinterpret_cast<const uint16_t *>(p)[j] << (j % 2 * 16);
+    }
+    return r;
+}
+
+// ---- sums over the lanes of a wave ----------------------------------------------------------------
+// Every one of G neighbouring lanes gets the sum of their values, added in an order that G fixes.
+template <int CTRL>
+__device__ inline float dpp(float v)
+{
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+
+__device__ inline float swap16_sum(float v)
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ inline float swap32_sum(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <int G>
+__device__ inline float lane_sum(float v)
+{
+    static_assert(G == 8 || G == 16 || G == 32 || G == 64, "lanes of one group");
+    v += dpp<0xB1>(v);                      // lane ^ 1
+    v += dpp<0x4E>(v);                      // lane ^ 2
+    v += dpp<0x141>(v);                     // 7 - lane in each eight: the other four
+    if (G >= 16) v += dpp<0x140>(v);        // 15 - lane in each sixteen: the other eight
+    if (G >= 32) v = swap16_sum(v);
+    if (G >= 64) v = swap32_sum(v);
+    return v;
+}
+
 inline bool known_type(int32_t t) { return t == SV3D_F32 || t == SV3D_F16 || t == SV3D_BF16; }
 inline int type_bytes(int32_t t) { return t == SV3D_F32 ? 4 : 2; }
 inline bool aligned(const void *p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }

@@ -11,36 +11,120 @@ namespace {
 using namespace sv3d;
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
 
-__device__ inline float wave_sum(float v)
+// ---- rows in registers ------------------------------------------------------------------------------
+// G threads share a row, each holds K packs of 16 bytes of it, G packs apart.  Rows shorter than a wave's packs
+// share the wave; rows longer than 64 threads hold take a workgroup, whose waves add up through LDS.
+template <class X>
+constexpr int kPack = 16 / (int)sizeof(X);
+
+template <int G>
+constexpr int kGroup = G > 256 ? G : 256;       // threads of the workgroup
+
+// The sum over the row's threads.  `part` is not written again before every thread has passed another row_sum on
+// another buffer, so one barrier is enough.
+template <int G>
+__device__ inline float row_sum(float v, float *part)
 {
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+    if (G <= 64) return lane_sum<(G < 64 ? G : 64)>(v);
+    v = lane_sum<64>(v);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = part[0];
+#pragma unroll
+    for (int w = 1; w < G / 64; ++w) v += part[w];
     return v;
 }
 
-// A wave per row, the row read three times.
-template <class X, class Y, class P>
-__global__ __launch_bounds__(kThreads) void layer_norm_forward_kernel(
-    const X *__restrict__ x, const P *__restrict__ weight, const P *__restrict__ bias, int64_t rows, int64_t cols,
-    int64_t x_stride, float eps, Y *__restrict__ y, float *__restrict__ mean, float *__restrict__ rstd)
+template <class T, int V>
+__device__ inline void store_pack(T *p, const float *v, int n)
 {
-    const int lane = threadIdx.x & 63;
-    for (int64_t row = (int64_t)blockIdx.x * kWaves + threadIdx.x / 64; row < rows; row += (int64_t)gridDim.x * kWaves) {
-        const X *xr = x + row * x_stride;
-        float s = 0.f;
-        for (int64_t c = lane; c < cols; c += 64) s += to_float(xr[c]);
-        const float mu = wave_sum(s) / (float)cols;
-        float q = 0.f;
-        for (int64_t c = lane; c < cols; c += 64) {
-            const float d = to_float(xr[c]) - mu;
-            q += d * d;
+    Pack<T, V> r;
+#pragma unroll
+    for (int j = 0; j < V; ++j) r.v[j] = from_float<T>(v[j]);
+    if (n >= V) {
+        *reinterpret_cast<Pack<T, V> *>(p) = r;
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (j < n) p[j] = r.v[j];
+}
+
+// weights of either type, kept in registers over all the rows of a thread
+template <class X, int V>
+__device__ inline void load_params(const void *p, bool f32, float missing, int c, int n, float *out)
+{
+    if (!p) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) out[j] = missing;
+    } else if (f32 || __is_same(X, float)) {
+        const auto r = load_words<float, V>((const float *)p + c, n);
+#pragma unroll
+        for (int j = 0; j < V; ++j) out[j] = r[j];
+    } else {
+        const auto r = load_words<X, V>((const X *)p + c, n);
+#pragma unroll
+        for (int j = 0; j < V; ++j) out[j] = r[j];
+    }
+}
+
+template <class X, class Y, int G, int K>
+__global__ __launch_bounds__(kGroup<G>) void layer_norm_forward_kernel(
+    const X *__restrict__ x, const void *__restrict__ weight, const void *__restrict__ bias, int params_f32, int cols,
+    int64_t rows, int64_t x_stride, float eps, Y *__restrict__ y, float *__restrict__ mean, float *__restrict__ rstd)
+{
+    constexpr int V = kPack<X>, R = kGroup<G> / G;
+    __shared__ float part[2][G > 64 ? G / 64 : 1];
+    const int lane = threadIdx.x % G;
+    const int64_t step = (int64_t)gridDim.x * R;
+    int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / G;
+    const float inv = 1.f / (float)cols;
+    Words<X, V> next[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int c = (k * G + lane) * V;
+        if (row < rows) next[k] = load_words<X, V>(x + row * x_stride + c, cols - c);
+    }
+    float w[K][V], b[K][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int c = (k * G + lane) * V;
+        load_params<X, V>(weight, params_f32, 1.f, c, cols - c, w[k]);
+        load_params<X, V>(bias, params_f32, 0.f, c, cols - c, b[k]);
+    }
+    for (; row < rows; row += step) {
+        float v[K][V], s = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                v[k][j] = next[k][j];
+                s += v[k][j];                       // zero behind the row's end
+            }
+        if (row + step < rows) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int c = (k * G + lane) * V;
+                next[k] = load_words<X, V>(x + (row + step) * x_stride + c, cols - c);
+            }
         }
-        const float r = 1.f / sqrtf(wave_sum(q) / (float)cols + eps);
-        Y *yr = y + row * cols;
-        for (int64_t c = lane; c < cols; c += 64) {
-            const float h = (to_float(xr[c]) - mu) * r;
-            yr[c] = from_float<Y>(h * (weight ? to_float(weight[c]) : 1.f) + (bias ? to_float(bias[c]) : 0.f));
+        const float mu = row_sum<G>(s, part[0]) * inv;
+        float q = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                v[k][j] -= mu;
+                q += (k * G + lane) * V + j < cols ? v[k][j] * v[k][j] : 0.f;
+            }
+        const float r = 1.f / sqrtf(row_sum<G>(q, part[1]) * inv + eps);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * G + lane) * V;
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[k][j] = v[k][j] * r * w[k][j] + b[k][j];
+            store_pack<Y, V>(y + row * cols + c, v[k], cols - c);
         }
         if (lane == 0) {
             if (mean) mean[row] = mu;
@@ -49,44 +133,231 @@ __global__ __launch_bounds__(kThreads) void layer_norm_forward_kernel(
     }
 }
 
-template <class X, class Y, class P>
-__global__ __launch_bounds__(kThreads) void layer_norm_dx_kernel(
-    const X *__restrict__ x, const Y *__restrict__ dy, const P *__restrict__ weight, const float *__restrict__ mean,
-    const float *__restrict__ rstd, int64_t rows, int64_t cols, int64_t x_stride, int64_t dy_stride, X *__restrict__ dx)
+// ---- rows beyond registers: a workgroup per row, which it reads three times ----------------------------
+constexpr int kLong = 1024;
+
+template <class X>
+__device__ inline float param(const void *p, bool f32, float missing, int c)
 {
-    const int lane = threadIdx.x & 63;
-    for (int64_t row = (int64_t)blockIdx.x * kWaves + threadIdx.x / 64; row < rows; row += (int64_t)gridDim.x * kWaves) {
+    return !p ? missing : f32 ? ((const float *)p)[c] : to_float(((const X *)p)[c]);
+}
+
+template <class X, class Y>
+__global__ __launch_bounds__(kLong) void layer_norm_forward_long_kernel(
+    const X *__restrict__ x, const void *__restrict__ weight, const void *__restrict__ bias, int params_f32, int cols,
+    int64_t rows, int64_t x_stride, float eps, Y *__restrict__ y, float *__restrict__ mean, float *__restrict__ rstd)
+{
+    __shared__ float part[2][kLong / 64];
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const X *xr = x + row * x_stride;
-        const Y *dr = dy + row * dy_stride;
-        const float mu = mean[row], r = rstd[row];
-        float su = 0.f, sh = 0.f;
-        for (int64_t c = lane; c < cols; c += 64) {
-            const float u = to_float(dr[c]) * (weight ? to_float(weight[c]) : 1.f);
-            su += u;
-            sh += u * ((to_float(xr[c]) - mu) * r);
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int c0 = threadIdx.x; c0 < cols; c0 += 4 * kLong)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (c0 + u * kLong < cols) s[u] += to_float(xr[c0 + u * kLong]);
+        const float mu = row_sum<kLong>((s[0] + s[1]) + (s[2] + s[3]), part[0]) / (float)cols;
+        float q[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int c0 = threadIdx.x; c0 < cols; c0 += 4 * kLong)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (c0 + u * kLong < cols) {
+                    const float d = to_float(xr[c0 + u * kLong]) - mu;
+                    q[u] += d * d;
+                }
+        const float r = 1.f / sqrtf(row_sum<kLong>((q[0] + q[1]) + (q[2] + q[3]), part[1]) / (float)cols + eps);
+        Y *yr = y + row * cols;
+        for (int c = threadIdx.x; c < cols; c += kLong) {
+            const float w = param<X>(weight, params_f32, 1.f, c), b = param<X>(bias, params_f32, 0.f, c);
+            yr[c] = from_float<Y>((to_float(xr[c]) - mu) * r * w + b);
         }
-        su = wave_sum(su) / (float)cols;
-        sh = wave_sum(sh) / (float)cols;
-        X *o = dx + row * cols;
-        for (int64_t c = lane; c < cols; c += 64) {
-            const float u = to_float(dr[c]) * (weight ? to_float(weight[c]) : 1.f);
-            o[c] = from_float<X>((u - su - (to_float(xr[c]) - mu) * r * sh) * r);
+        if (threadIdx.x == 0) {
+            if (mean) mean[row] = mu;
+            if (rstd) rstd[row] = r;
         }
     }
 }
 
-// dweight and dbias: a thread per column adds up a slice of the rows ...
+// ---- backward, rows in registers --------------------------------------------------------------------
+// One pass over x and dy: dx, and the weights' gradients of the workgroup's rows, which stay in registers until its last
+// row, are added up over the rows that the workgroup has at a time and go to `part` [workgroup][2][cols].  x and dy
+// are held as they were loaded and converted where they are used: with the weight and the two gradients in registers
+// there is no room for the values in fp32 as well, and arithmetic is not what this waits for.
+constexpr int kBack = 1024;
+
+template <class X, class Y, int G, int K>
+__global__ __launch_bounds__(kBack) void layer_norm_backward_kernel(
+    const X *__restrict__ x, const Y *__restrict__ dy, const void *__restrict__ weight, int params_f32, int cols, int64_t rows,
+    const float *__restrict__ mean, const float *__restrict__ rstd, int64_t x_stride, int64_t dy_stride, X *__restrict__ dx,
+    float *__restrict__ part)
+{
+    constexpr int V = kPack<X>, R = kBack / G, E = K * V;
+    __shared__ float both[2][2][kBack / 64];
+    const int lane = threadIdx.x % G, wave = threadIdx.x / 64;
+    const int64_t step = (int64_t)gridDim.x * R;
+    int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / G;
+    const float inv = 1.f / (float)cols;
+    Words<X, V> nx[K];
+    Words<Y, V> nd[K];
+    float nmu, nr;
+    // a row behind the last one has dy = 0 and adds nothing anywhere
+    const auto fetch = [&](int64_t at) {
+        const bool there = at < rows;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * G + lane) * V, n = there ? cols - c : 0;
+            nx[k] = load_words<X, V>(x + at * x_stride + c, n);
+            nd[k] = load_words<Y, V>(dy + at * dy_stride + c, n);
+        }
+        nmu = there ? mean[at] : 0.f;
+        nr = there ? rstd[at] : 0.f;
+    };
+    fetch(row);
+    float w[E], dw[E], db[E];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int c = (k * G + lane) * V;
+        load_params<X, V>(weight, params_f32, 1.f, c, cols - c, w + k * V);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
+    int turn = 0;
+    for (int64_t base = (int64_t)blockIdx.x * R; base < rows; base += step, row += step, turn ^= 1) {
+        Words<X, V> cx[K];
+        Words<Y, V> cd[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            cx[k] = nx[k];
+            cd[k] = nd[k];
+        }
+        const float mu = nmu, r = nr;
+        if (base + step < rows) fetch(row + step);
+        float su = 0.f, sh = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float d = cd[e / V][e % V];       // zero behind the row's end, and so is all that it enters
+            const float h = (cx[e / V][e % V] - mu) * r, u = d * w[e];
+            dw[e] += d * h;
+            db[e] += d;
+            su += u;
+            sh += u * h;
+        }
+        if (!dx) continue;
+        su = lane_sum<(G < 64 ? G : 64)>(su);
+        sh = lane_sum<(G < 64 ? G : 64)>(sh);
+        if constexpr (G > 64) {
+            // both sums with one barrier; the buffers of two turns alternate
+            if ((threadIdx.x & 63) == 0) {
+                both[turn][0][wave] = su;
+                both[turn][1][wave] = sh;
+            }
+            __syncthreads();
+            const int first = threadIdx.x / G * (G / 64);
+            su = both[turn][0][first];
+            sh = both[turn][1][first];
+#pragma unroll
+            for (int i = 1; i < G / 64; ++i) {
+                su += both[turn][0][first + i];
+                sh += both[turn][1][first + i];
+            }
+        }
+        su *= inv;
+        sh *= inv;
+        if (row >= rows) continue;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * G + lane) * V;
+            float o[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float h = (cx[k][j] - mu) * r, u = cd[k][j] * w[k * V + j];
+                o[j] = (u - su - h * sh) * r;
+            }
+            store_pack<X, V>(dx + row * cols + c, o, cols - c);
+        }
+    }
+    if (!part) return;
+    // the rows that share a wave, then the others by halves
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+#pragma unroll
+        for (int d = G; d < 64; d *= 2) {
+            dw[e] += __shfl_xor(dw[e], d);
+            db[e] += __shfl_xor(db[e], d);
+        }
+    }
+    constexpr int kTeam = G < 64 ? 64 : G, kHalf = kBack / kTeam / 2;
+    const int team = threadIdx.x / kTeam;
+    const bool first = threadIdx.x % kTeam < G;
+    if constexpr (kHalf > 0) {
+        __shared__ float fold[kHalf][E][G];
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            float(&acc)[E] = which ? db : dw;
+            for (int half = kHalf; half > 0; half /= 2) {
+                __syncthreads();
+                if (first && team >= half && team < 2 * half)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) fold[team - half][e][lane] = acc[e];
+                __syncthreads();
+                if (first && team < half)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] += fold[team][e][lane];
+            }
+        }
+    }
+    if (team != 0 || !first) return;
+    float *out = part + (int64_t)blockIdx.x * 2 * cols;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int c = (k * G + lane) * V;
+        store_pack<float, V>(out + c, dw + k * V, cols - c);
+        store_pack<float, V>(out + cols + c, db + k * V, cols - c);
+    }
+}
+
+// Rows beyond registers: a workgroup per row, which it reads twice.
+template <class X, class Y>
+__global__ __launch_bounds__(kLong) void layer_norm_dx_long_kernel(
+    const X *__restrict__ x, const Y *__restrict__ dy, const void *__restrict__ weight, int params_f32, int cols, int64_t rows,
+    const float *__restrict__ mean, const float *__restrict__ rstd, int64_t x_stride, int64_t dy_stride, X *__restrict__ dx)
+{
+    __shared__ float part[2][kLong / 64];
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const X *xr = x + row * x_stride;
+        const Y *dr = dy + row * dy_stride;
+        const float mu = mean[row], r = rstd[row];
+        float su[2] = {0.f, 0.f}, sh[2] = {0.f, 0.f};
+        for (int c0 = threadIdx.x; c0 < cols; c0 += 2 * kLong)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int c = c0 + t * kLong;
+                if (c >= cols) break;
+                const float u = to_float(dr[c]) * param<X>(weight, params_f32, 1.f, c);
+                su[t] += u;
+                sh[t] += u * ((to_float(xr[c]) - mu) * r);
+            }
+        const float mu_u = row_sum<kLong>(su[0] + su[1], part[0]) / (float)cols;
+        const float mu_uh = row_sum<kLong>(sh[0] + sh[1], part[1]) / (float)cols;
+        X *o = dx + row * cols;
+        for (int c = threadIdx.x; c < cols; c += kLong) {
+            const float w = param<X>(weight, params_f32, 1.f, c);
+            o[c] = from_float<X>((to_float(dr[c]) * w - mu_u - (to_float(xr[c]) - mu) * r * mu_uh) * r);
+        }
+    }
+}
+
+// dweight and dbias of such rows: a thread per column adds up a slice of the rows
 constexpr int kSlices = 64;
 
 template <class X, class Y>
 __global__ __launch_bounds__(kThreads) void layer_norm_slices_kernel(
     const X *__restrict__ x, const Y *__restrict__ dy, const float *__restrict__ mean, const float *__restrict__ rstd,
-    int64_t rows, int64_t cols, int64_t x_stride, int64_t dy_stride, float *__restrict__ part)
+    int64_t rows, int cols, int64_t x_stride, int64_t dy_stride, float *__restrict__ part)
 {
-    const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int c = blockIdx.x * kThreads + threadIdx.x;
     if (c >= cols) return;
     float w = 0.f, b = 0.f;
-    for (int64_t row = blockIdx.y; row < rows; row += kSlices) {
+    for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
         const float d = to_float(dy[row * dy_stride + c]);
         w += d * ((to_float(x[row * x_stride + c]) - mean[row]) * rstd[row]);
         b += d;
@@ -95,27 +366,26 @@ __global__ __launch_bounds__(kThreads) void layer_norm_slices_kernel(
     part[(2 * (int64_t)blockIdx.y + 1) * cols + c] = b;
 }
 
-// ... and then the slices
+// The sum over the `count` partial sums: 16 columns of one of the two gradients per workgroup, 64 threads each.
 template <class P>
-__global__ __launch_bounds__(kThreads) void layer_norm_join_kernel(const float *__restrict__ part, int64_t cols,
-                                                                   P *__restrict__ dweight, P *__restrict__ dbias)
+__global__ __launch_bounds__(1024) void layer_norm_join_kernel(const float *__restrict__ part, int count, int cols,
+                                                               P *__restrict__ dweight, P *__restrict__ dbias)
 {
-    const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (c >= cols) return;
-    float w = 0.f, b = 0.f;
-    for (int s = 0; s < kSlices; ++s) {
-        w += part[(2 * (int64_t)s) * cols + c];
-        b += part[(2 * (int64_t)s + 1) * cols + c];
-    }
-    if (dweight) dweight[c] = from_float<P>(w);
-    if (dbias) dbias[c] = from_float<P>(b);
-}
-
-// workgroups for a wave per row; beyond the cap (a launch holds fewer than 2^32 threads) a wave takes several rows
-uint32_t row_blocks(int64_t rows)
-{
-    const int64_t n = (rows + kWaves - 1) / kWaves;
-    return (uint32_t)(n < (1 << 20) ? n : (1 << 20));
+    __shared__ float fold[64][17];
+    P *out = blockIdx.y ? dbias : dweight;
+    if (!out) return;
+    const int c = blockIdx.x * 16 + threadIdx.x % 16, slice = threadIdx.x / 16;
+    float s = 0.f;
+    if (c < cols)
+        for (int i = slice; i < count; i += 64) s += part[(2 * (int64_t)i + blockIdx.y) * cols + c];
+    fold[slice][threadIdx.x % 16] = s;
+    __syncthreads();
+    if (threadIdx.x >= 256) return;
+    // 16 lanes for each of the 16 columns
+    const int column = threadIdx.x / 16, l = threadIdx.x % 16;
+    s = (fold[l][column] + fold[l + 16][column]) + (fold[l + 32][column] + fold[l + 48][column]);
+    s = lane_sum<16>(s);
+    if (l == 0 && blockIdx.x * 16 + column < cols) out[blockIdx.x * 16 + column] = from_float<P>(s);
 }
 
 int check(const sv3d_layer_norm_params *p)
@@ -128,22 +398,96 @@ int check(const sv3d_layer_norm_params *p)
     return SV3D_OK;
 }
 
-// calls f(x, y, param) with null pointers of the element types
+// Threads per row and packs per thread that hold `cols` columns, as a call f(G, K): the fewest threads that do with at
+// most two packs each up to 64 threads (rows that share a wave or have one to themselves add up without a barrier), then
+// 256 threads, then 1024; f(0, 0) beyond.
+template <int G_, int K_>
+struct Shape {
+    static constexpr int G = G_, K = K_;
+};
+
 template <class X, class F>
-int with_types_of(const sv3d_layer_norm_params *p, F f)
+int with_shape(int64_t cols, F f)
 {
-    const bool y32 = p->y_type == SV3D_F32, p32 = p->param_type == SV3D_F32;
-    if (y32 && p32) return f((X *)nullptr, (float *)nullptr, (float *)nullptr);
-    if (y32) return f((X *)nullptr, (float *)nullptr, (X *)nullptr);
-    if (p32) return f((X *)nullptr, (X *)nullptr, (float *)nullptr);
-    return f((X *)nullptr, (X *)nullptr, (X *)nullptr);
+    const int64_t packs = (cols + kPack<X> - 1) / kPack<X>;
+    if (packs <= 8) return f(Shape<8, 1>());
+    if (packs <= 16) return f(Shape<16, 1>());
+    if (packs <= 32) return f(Shape<32, 1>());
+    if (packs <= 64) return f(Shape<64, 1>());
+    if (packs <= 128) return f(Shape<64, 2>());
+    if (packs <= 256) return f(Shape<256, 1>());
+    if (packs <= 512) return f(Shape<256, 2>());
+    if (packs <= 1024) return f(Shape<256, 4>());
+    if (packs <= 2048) return f(Shape<1024, 2>());
+    if constexpr (kPack<X> == 4)
+        if (packs <= 4096) return f(Shape<1024, 4>());
+    return f(Shape<0, 0>());
 }
 
-template <class F>
-int with_types(const sv3d_layer_norm_params *p, F f)
+// The same for the backward, which holds five values for each element: eight elements per thread, up to 8192 columns
+// (sixteen do not fit the 128 registers of a thread in a workgroup of 1024).
+template <class X, class F>
+int with_back_shape(int64_t cols, F f)
 {
-    if (p->x_type == SV3D_F32) return f((float *)nullptr, (float *)nullptr, (float *)nullptr);
-    return p->x_type == SV3D_F16 ? with_types_of<f16>(p, f) : with_types_of<bf16>(p, f);
+    const int64_t packs = (cols + kPack<X> - 1) / kPack<X>;
+    constexpr int K = 8 / kPack<X>;
+    if (packs <= 8) return f(Shape<8, 1>());
+    if (packs <= 16) return f(Shape<16, 1>());
+    if (packs <= 32) return f(Shape<32, 1>());
+    if (packs <= 64) return f(Shape<64, 1>());
+    if constexpr (K == 2)
+        if (packs <= 128) return f(Shape<64, 2>());
+    if (packs <= 128 * K) return f(Shape<128, K>());
+    if (packs <= 256 * K) return f(Shape<256, K>());
+    if (packs <= 512 * K) return f(Shape<512, K>());
+    if (packs <= 1024 * K) return f(Shape<1024, K>());
+    return f(Shape<0, 0>());
+}
+
+// A workgroup for each set of rows, but no more than the device holds at once: more rows are taken in turn, with the
+// weights in registers and the next row's load on its way.
+uint32_t persistent_groups(int64_t rows, int rows_per_group, int threads)
+{
+    const int64_t want = (rows + rows_per_group - 1) / rows_per_group, fit = 256 * (2048 / threads);
+    return (uint32_t)(want < fit ? want : fit);
+}
+
+template <class X, class F>
+int with_output(const sv3d_layer_norm_params *p, F f)
+{
+    return p->y_type == SV3D_F32 ? f((X *)nullptr, (float *)nullptr) : f((X *)nullptr, (X *)nullptr);
+}
+
+// calls f(x, y) with null pointers of the element types
+template <class F>
+int with_xy(const sv3d_layer_norm_params *p, F f)
+{
+    if (p->x_type == SV3D_F32) return f((float *)nullptr, (float *)nullptr);
+    return p->x_type == SV3D_F16 ? with_output<f16>(p, f) : with_output<bf16>(p, f);
+}
+
+// Workgroups of the backward, each of which leaves one partial sum of dweight and dbias: two for each CU, enough to fill
+// the device and few enough that the partial sums are a small part of what is read.
+constexpr int kBackGroups = 512;
+
+template <class X>
+int partial_sums(const sv3d_layer_norm_params *p)
+{
+    return with_back_shape<X>(p->cols, [&](auto shape) {
+        constexpr int G = decltype(shape)::G;
+        if constexpr (G == 0) {
+            return (int)(p->rows < kSlices ? p->rows : kSlices);
+        } else {
+            constexpr int R = kBack / G;
+            const int64_t want = (p->rows + R - 1) / R;
+            return (int)(want < kBackGroups ? want : kBackGroups);
+        }
+    });
+}
+
+int partial_sums(const sv3d_layer_norm_params *p)
+{
+    return p->x_type == SV3D_F32 ? partial_sums<float>(p) : partial_sums<f16>(p);
 }
 
 }  // namespace
@@ -154,14 +498,23 @@ extern "C" int sv3d_layer_norm_forward(const sv3d_layer_norm_params *p, const vo
     if (const int st = check(p)) return st;
     if (p->rows == 0) return SV3D_OK;
     if (!x || !y) return SV3D_ERR_INVALID_ARG;
-    return with_types(p, [&](auto *X, auto *Y, auto *P) {
-        using XT = std::remove_pointer_t<decltype(X)>;
-        using YT = std::remove_pointer_t<decltype(Y)>;
-        using PT = std::remove_pointer_t<decltype(P)>;
-        hipLaunchKernelGGL((layer_norm_forward_kernel<XT, YT, PT>), dim3(row_blocks(p->rows)),
-                           dim3(kThreads), 0, (hipStream_t)stream, (const XT *)x, (const PT *)weight, (const PT *)bias,
-                           p->rows, p->cols, p->x_stride, p->eps, (YT *)y, mean, rstd);
-        return launch_status();
+    return with_xy(p, [&](auto *xt, auto *yt) {
+        using X = std::remove_pointer_t<decltype(xt)>;
+        using Y = std::remove_pointer_t<decltype(yt)>;
+        return with_shape<X>(p->cols, [&](auto shape) {
+            constexpr int G = decltype(shape)::G, K = decltype(shape)::K;
+            const int f32 = p->param_type == SV3D_F32, cols = (int)p->cols;
+            if constexpr (G == 0)
+                hipLaunchKernelGGL((layer_norm_forward_long_kernel<X, Y>), dim3(persistent_groups(p->rows, 1, kLong)),
+                                   dim3(kLong), 0, (hipStream_t)stream, (const X *)x, weight, bias, f32, cols, p->rows,
+                                   p->x_stride, p->eps, (Y *)y, mean, rstd);
+            else
+                hipLaunchKernelGGL((layer_norm_forward_kernel<X, Y, G, K>),
+                                   dim3(persistent_groups(p->rows, kGroup<G> / G, kGroup<G>)), dim3(kGroup<G>), 0,
+                                   (hipStream_t)stream, (const X *)x, weight, bias, f32, cols, p->rows, p->x_stride, p->eps,
+                                   (Y *)y, mean, rstd);
+            return launch_status();
+        });
     });
 }
 
@@ -169,7 +522,7 @@ extern "C" int sv3d_layer_norm_workspace(const sv3d_layer_norm_params *p, size_t
 {
     if (!bytes) return SV3D_ERR_INVALID_ARG;
     if (const int st = check(p)) return st;
-    *bytes = (size_t)2 * kSlices * p->cols * sizeof(float);
+    *bytes = (size_t)2 * partial_sums(p) * p->cols * sizeof(float);
     return SV3D_OK;
 }
 
@@ -182,32 +535,47 @@ extern "C" int sv3d_layer_norm_backward(const sv3d_layer_norm_params *p, const v
     if (p->dy_stride < 0) return SV3D_ERR_INVALID_ARG;
     if (p->rows > 0 && (!x || !dy || !mean || !rstd)) return SV3D_ERR_INVALID_ARG;
     const bool params = dweight || dbias;
-    if (params) {
+    if (params && p->rows > 0) {
         size_t need = 0;
         sv3d_layer_norm_workspace(p, &need);
         if (!workspace || !aligned(workspace, 16)) return SV3D_ERR_INVALID_ARG;
         if (workspace_bytes < need) return SV3D_ERR_WORKSPACE;
     }
-    return with_types(p, [&](auto *X, auto *Y, auto *P) {
-        using XT = std::remove_pointer_t<decltype(X)>;
-        using YT = std::remove_pointer_t<decltype(Y)>;
-        using PT = std::remove_pointer_t<decltype(P)>;
-        if (dx && p->rows > 0) {
-            hipLaunchKernelGGL((layer_norm_dx_kernel<XT, YT, PT>), dim3(row_blocks(p->rows)),
-                               dim3(kThreads), 0, (hipStream_t)stream, (const XT *)x, (const YT *)dy, (const PT *)weight,
-                               mean, rstd, p->rows, p->cols, p->x_stride, p->dy_stride, (XT *)dx);
-            if (const int st = launch_status()) return st;
-        }
-        if (params) {
-            const uint32_t blocks = (uint32_t)((p->cols + kThreads - 1) / kThreads);
-            hipLaunchKernelGGL((layer_norm_slices_kernel<XT, YT>), dim3(blocks, kSlices), dim3(kThreads), 0,
-                               (hipStream_t)stream, (const XT *)x, (const YT *)dy, mean, rstd, p->rows, p->cols,
-                               p->x_stride, p->dy_stride, (float *)workspace);
-            if (const int st = launch_status()) return st;
-            hipLaunchKernelGGL((layer_norm_join_kernel<PT>), dim3(blocks), dim3(kThreads), 0, (hipStream_t)stream,
-                               (const float *)workspace, p->cols, (PT *)dweight, (PT *)dbias);
-            return launch_status();
-        }
-        return (int)SV3D_OK;
-    });
+    const int cols = (int)p->cols, count = partial_sums(p), f32 = p->param_type == SV3D_F32;
+    float *part = params ? (float *)workspace : nullptr;
+    hipStream_t s = (hipStream_t)stream;
+    if (p->rows > 0 && (dx || params)) {
+        const int st = with_xy(p, [&](auto *xt, auto *yt) {
+            using X = std::remove_pointer_t<decltype(xt)>;
+            using Y = std::remove_pointer_t<decltype(yt)>;
+            return with_back_shape<X>(p->cols, [&](auto shape) {
+                constexpr int G = decltype(shape)::G, K = decltype(shape)::K;
+                if constexpr (G > 0) {
+                    hipLaunchKernelGGL((layer_norm_backward_kernel<X, Y, G, K>), dim3(count), dim3(kBack), 0, s,
+                                       (const X *)x, (const Y *)dy, weight, f32, cols, p->rows, mean, rstd, p->x_stride,
+                                       p->dy_stride, (X *)dx, part);
+                } else {
+                    if (dx)
+                        hipLaunchKernelGGL((layer_norm_dx_long_kernel<X, Y>), dim3(persistent_groups(p->rows, 1, kLong)),
+                                           dim3(kLong), 0, s, (const X *)x, (const Y *)dy, weight, f32, cols, p->rows, mean,
+                                           rstd, p->x_stride, p->dy_stride, (X *)dx);
+                    if (part)
+                        hipLaunchKernelGGL((layer_norm_slices_kernel<X, Y>), dim3((cols + kThreads - 1) / kThreads, count),
+                                           dim3(kThreads), 0, s, (const X *)x, (const Y *)dy, mean, rstd, p->rows, cols,
+                                           p->x_stride, p->dy_stride, part);
+                }
+                return launch_status();
+            });
+        });
+        if (st) return st;
+    }
+    if (!params) return SV3D_OK;
+    const dim3 grid((cols + 15) / 16, 2);
+    if (p->param_type == SV3D_F32)
+        hipLaunchKernelGGL(layer_norm_join_kernel<float>, grid, dim3(1024), 0, s, part, count, cols, (float *)dweight, (float *)dbias);
+    else if (p->param_type == SV3D_F16)
+        hipLaunchKernelGGL(layer_norm_join_kernel<f16>, grid, dim3(1024), 0, s, part, count, cols, (f16 *)dweight, (f16 *)dbias);
+    else
+        hipLaunchKernelGGL(layer_norm_join_kernel<bf16>, grid, dim3(1024), 0, s, part, count, cols, (bf16 *)dweight, (bf16 *)dbias);
+    return launch_status();
 }
