@@ -17,6 +17,7 @@ constexpr int kChunk = 2048;        // elements of one workgroup of the update
 constexpr int kBlock = SV3D_STATE_BLOCK;
 constexpr int kSumChunk = 4096;
 constexpr int kSumGroups = 1024;
+constexpr float kSmallest = 0x1p-126f;
 
 // ---- the norm: sums of squares --------------------------------------------------------------------
 // Squares and sums in double: a square of an fp32 number neither overflows nor is rounded there, and the order of
@@ -32,23 +33,29 @@ template <class T>
 __global__ __launch_bounds__(kThreads) void grad_square_sums_kernel(SumTable t, double *__restrict__ sums)
 {
     __shared__ double part[kThreads / 64];
-    double acc = 0.0;
+    double acc[4] = {0.0, 0.0, 0.0, 0.0};
     int k = 0;
     for (int chunk = blockIdx.x; chunk < t.first[t.count]; chunk += gridDim.x) {
         while (chunk >= t.first[k + 1]) ++k;
         const T *g = (const T *)t.grad[k];
-        const int64_t at = (int64_t)(chunk - t.first[k]) * kSumChunk, end = min(at + kSumChunk, t.numel[k]);
-        for (int64_t i = at + threadIdx.x; i < end; i += kThreads) {
-            const double v = (double)to_float(g[i]);
-            acc += v * v;
+        const int64_t at = (int64_t)(chunk - t.first[k]) * kSumChunk;
+        const int left = (int)min(t.numel[k] - at, (int64_t)kSumChunk);
+        constexpr int V = 16 / (int)sizeof(T);
+#pragma unroll
+        for (int u = 0; u < kSumChunk / (kThreads * V); ++u) {
+            const int o = (u * kThreads + threadIdx.x) * V;
+            const auto w = load_words<T, V>(g + at + o, left - o);
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j & 3] += (double)w[j] * (double)w[j];
         }
     }
-    for (int d = 32; d > 0; d >>= 1) acc += __shfl_xor(acc, d);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = acc;
+    double sum = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < kThreads / 64; ++w) acc += part[w];
-        sums[blockIdx.x] = acc;
+        for (int w = 1; w < kThreads / 64; ++w) sum += part[w];
+        sums[blockIdx.x] = sum;
     }
 }
 
@@ -122,59 +129,46 @@ __device__ inline uint32_t dither(uint32_t element, uint32_t key)
 
 __device__ inline float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// A magnitude t < 2^(17 or 8) to a code with three mantissa bits whose smallest normal value is 2^LOWEST: 20 bits
-// of the fp32 mantissa fall off, after `bits` (16 of them, and half a one) has been added to them.  Below 2^LOWEST
-// the codes are evenly spaced, as they are in the octave above it, so t is moved there.
-template <int LOWEST>
-__device__ inline uint32_t cut(float t, uint32_t bits)
-{
-    const bool small = t < power_of_two(LOWEST);
-    t += small ? power_of_two(LOWEST) : 0.f;
-    return ((__float_as_uint(t) + (bits << 4) + 8u) >> 20) - ((126u + LOWEST) << 3) - (small ? 8u : 0u);
-}
-
-// what a moment contributes to its block's exponent: an infinity or NaN does not
-__device__ inline float finite_magnitude(float v) { return fabsf(v) < INFINITY ? fabsf(v) : 0.f; }
-
+// A code is the upper bits of a float32 whose exponent field is as narrow as the code's: with a block's values scaled so
+// that the code's smallest exponent meets float32's, bits 20 and up of a value ARE its code, its subnormal codes included
+// (float32's own subnormal numbers), and the dither (16 bits and half a one) goes in below before they are cut off.
+//   first:  field = exponent + 7,  sign in bit 31;     second: field = exponent + 15
 constexpr int kFirstBias = 134, kSecondBias = 142;      // a block's largest value lands in [2^7, 2^8) and [2^15, 2^16)
 constexpr int kFirstFloor = 20, kSecondFloor = 34;      // so that every value is a normal number, also as bf16
+constexpr int kFirstField = 127 - 7, kSecondField = 127 - 15;
 
-__device__ inline uint32_t block_exponent(float largest, int floor) { return (uint32_t)max((int)(__float_as_uint(largest) >> 23), floor); }
+// what to multiply by two to the power of, from a value to its code's place; a byte below the lowest that is ever
+// written (fresh state: 0) counts as that one
+__device__ inline int first_power(uint32_t e) { return kFirstBias - kFirstField - max((int)e, kFirstFloor); }
+__device__ inline int second_power(uint32_t e) { return kSecondBias - kSecondField - max((int)e, kSecondFloor); }
 
-__device__ inline uint32_t encode_first(float m, float scale, uint32_t bits)
+__device__ inline uint32_t block_exponent(uint32_t largest_bits, int floor) { return (uint32_t)max((int)(largest_bits >> 23), floor); }
+
+constexpr uint32_t kInfinity = 0x7f800000u;
+__device__ inline uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// what a moment contributes to its block's exponent: an infinity or NaN does not
+__device__ inline uint32_t finite_bits(float v) { return magnitude_bits(v) < kInfinity ? magnitude_bits(v) : 0u; }
+
+// `low`: the dither bits in place, (bits << 4) + 8
+__device__ inline uint32_t encode_first(float m, int power, uint32_t low)
 {
-    const float a = fabsf(m);
-    const uint32_t code = a < INFINITY ? cut<-6>(a * scale, bits) : 0x7fu;
-    return code | (__float_as_uint(m) >> 31 << 7);
+    const uint32_t q = (__float_as_uint(ldexpf(m, power)) + low) >> 20;
+    return (magnitude_bits(m) < kInfinity ? q & 0x7fu : 0x7fu) | (q >> 4 & 0x80u);
 }
 
-__device__ inline uint32_t encode_second(float v, float scale, uint32_t bits)
+__device__ inline uint32_t encode_second(float v, int power, uint32_t low)
 {
-    if (!(v < INFINITY)) return 0xffu;
-    const uint32_t code = cut<-14>(v * scale, bits);
-    return v > 0.f ? max(code, 1u) : code;
+    const uint32_t q = (__float_as_uint(ldexpf(v, power)) + low) >> 20;
+    return !(v < INFINITY) ? 0xffu : v > 0.f ? max(q, 1u) : q;
 }
 
-template <int LOWEST>
-__device__ inline float magnitude(uint32_t code)
+__device__ inline float decode_first(uint32_t code, int power)
 {
-    const bool small = code < 8u;
-    const float t = __uint_as_float((code + ((126u + LOWEST) << 3) + (small ? 8u : 0u)) << 20);
-    return t - (small ? power_of_two(LOWEST) : 0.f);
+    const float v = ldexpf(__uint_as_float((code & 0x7fu) << 20 | (code & 0x80u) << 24), -power);
+    return (code & 0x7fu) == 0x7fu ? NAN : v;
 }
 
-__device__ inline float decode_first(uint32_t code, float unit)
-{
-    const uint32_t c = code & 0x7fu;
-    const float a = c == 0x7fu ? NAN : magnitude<-6>(c) * unit;
-    return code & 0x80u ? -a : a;
-}
-
-__device__ inline float decode_second(uint32_t code, float unit) { return code == 0xffu ? NAN : magnitude<-14>(code) * unit; }
-
-// the power of two of a block's codes; a byte below the lowest that is ever written (fresh state: 0) counts as that one
-__device__ inline float first_unit(uint32_t e) { return power_of_two(max((int)e, kFirstFloor) - kFirstBias); }
-__device__ inline float second_unit(uint32_t e) { return power_of_two(max((int)e, kSecondFloor) - kSecondBias); }
+__device__ inline float decode_second(uint32_t code, int power) { return code == 0xffu ? NAN : ldexpf(__uint_as_float(code << 20), -power); }
 
 // ---- the update --------------------------------------------------------------------------------------
 struct Entry {
@@ -196,91 +190,144 @@ struct Betas {
     float b1, c1, b2, c2, eps;          // c = 1 - b, taken in double
 };
 
-// products and sums as they stand, each rounded: the same moments on every path
+// Products and sums of the moments as they stand, each rounded: the same bits on every path.  The root and the
+// quotient are the hardware's (off by one unit in the last place where the exact ones are off by half); it takes numbers
+// below the normal ones for zero, hence the lower end.
 __device__ inline float step_of(float &m, float &v, float g, const Betas &b, const Factors &f)
 {
     m = __fadd_rn(__fmul_rn(b.b1, m), __fmul_rn(b.c1, g));
     v = __fadd_rn(__fmul_rn(b.b2, v), __fmul_rn(b.c2, __fmul_rn(g, g)));
-    return f.rate * (m / (sqrtf(v) * f.root + b.eps));
+    const float root = __builtin_amdgcn_sqrtf(v < kSmallest ? kSmallest : v);       // NaN stays
+    return f.rate * (m * __builtin_amdgcn_rcpf(root * f.root + b.eps));
+}
+
+// The tensor of chunk `chunk`: the lanes look at the 64 table entries at once.
+__device__ inline int tensor_of(const int32_t *first, int count, int chunk)
+{
+    const int lane = threadIdx.x & 63;
+    return __popcll(__ballot(lane < count && chunk >= first[lane + 1]));
 }
 
 template <class T>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(Table t, Betas b, const Factors *__restrict__ factors)
 {
-    int k = 0;
-    while ((int)blockIdx.x >= t.first[k + 1]) ++k;
+    const int k = __builtin_amdgcn_readfirstlane(tensor_of(t.first, t.count, blockIdx.x));
     const Entry e = t.t[k];
     const Factors f = factors[t.order[k]];
     if (f.skip) return;
-    const int64_t at = (int64_t)((int)blockIdx.x - t.first[k]) * kChunk, end = min(at + kChunk, e.numel);
-    T *p = (T *)e.param;
-    const T *g = (const T *)e.grad;
-    float *em = (float *)e.exp_avg, *ev = (float *)e.exp_avg_sq;
-    for (int64_t i = at + threadIdx.x; i < end; i += kThreads) {
-        float m = em[i], v = ev[i];
-        const float s = step_of(m, v, to_float(g[i]) * f.grad, b, f);
-        em[i] = m;
-        ev[i] = v;
-        p[i] = from_float<T>(to_float(p[i]) * f.decay - s);
+    constexpr int V = 4, U = kChunk / (kThreads * V);
+    const int64_t at = (int64_t)((int)blockIdx.x - t.first[k]) * kChunk + threadIdx.x * V;
+    T *p = (T *)e.param + at;
+    const T *g = (const T *)e.grad + at;
+    float *em = (float *)e.exp_avg + at, *ev = (float *)e.exp_avg_sq + at;
+    const int left = (int)min(e.numel - at, (int64_t)kChunk);
+    Words<T, V> wp[U], wg[U];
+    Words<float, V> wm[U], wv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int o = u * kThreads * V, n = left - o;
+        wg[u] = load_words<T, V>(g + o, n);
+        wm[u] = load_words<float, V>(em + o, n);
+        wv[u] = load_words<float, V>(ev + o, n);
+        wp[u] = load_words<T, V>(p + o, n);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int o = u * kThreads * V, n = left - o;
+        float np[V], nm[V], nv[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            nm[j] = wm[u][j];
+            nv[j] = wv[u][j];
+            const float s = step_of(nm[j], nv[j], wg[u][j] * f.grad, b, f);
+            np[j] = wp[u][j] * f.decay - s;
+        }
+        store_pack<float, V>(em + o, nm, n);
+        store_pack<float, V>(ev + o, nv, n);
+        store_pack<T, V>(p + o, np, n);
     }
 }
 
-// 16 lanes share a block of 128 elements, eight each
+// the largest of 16 neighbouring lanes, in each of them
+__device__ inline uint32_t largest16(uint32_t v)
+{
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true));
+}
+
+// 16 lanes share a block of 128 elements, eight each.  Elements behind the end are zero: they add nothing to the
+// block's exponents and are not stored.
 template <class T>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(Table t, Betas b, const Factors *__restrict__ factors)
 {
-    int k = 0;
-    while ((int)blockIdx.x >= t.first[k + 1]) ++k;
+    const int k = __builtin_amdgcn_readfirstlane(tensor_of(t.first, t.count, blockIdx.x));
     const Entry e = t.t[k];
     const Factors f = factors[t.order[k]];
     if (f.skip) return;
-    const int64_t i0 = (int64_t)((int)blockIdx.x - t.first[k]) * kChunk + threadIdx.x * 8, block = i0 / kBlock;
-    const bool live = i0 < e.numel;
-    T *p = (T *)e.param;
-    const T *g = (const T *)e.grad;
-    uint8_t *cm = (uint8_t *)e.exp_avg, *cv = (uint8_t *)e.exp_avg_sq;
-    const float um = live ? first_unit(e.scales[2 * block]) : 0.f;
-    const float uv = live ? second_unit(e.scales[2 * block + 1]) : 0.f;
-    float m[8], v[8], top_m = 0.f, top_v = 0.f;
-    for (int j = 0; j < 8; ++j) {
-        const int64_t i = i0 + j;
-        m[j] = v[j] = 0.f;
-        if (i >= e.numel) continue;
-        m[j] = decode_first(cm[i], um);
-        v[j] = decode_second(cv[i], uv);
-        const float s = step_of(m[j], v[j], to_float(g[i]) * f.grad, b, f);
-        p[i] = from_float<T>(to_float(p[i]) * f.decay - s);
-        top_m = fmaxf(top_m, finite_magnitude(m[j]));
-        top_v = fmaxf(top_v, finite_magnitude(v[j]));
+    constexpr int V = 8;
+    const int64_t at = (int64_t)((int)blockIdx.x - t.first[k]) * kChunk + threadIdx.x * V;
+    // the 16 lanes of a block stay or go together: each of them passes on what others found
+    if (at - (int)(threadIdx.x & 15) * V >= e.numel) return;
+    const int n = (int)max(min(e.numel - at, (int64_t)V), (int64_t)0);
+    T *p = (T *)e.param + at;
+    const T *g = (const T *)e.grad + at;
+    uint8_t *cm = (uint8_t *)e.exp_avg + at, *cv = (uint8_t *)e.exp_avg_sq + at;
+    uint8_t *scales = e.scales + at / kBlock * 2;
+    const auto wg = load_words<T, V>(g, n);
+    const auto bm = load_words<uint8_t, V>(cm, n), bv = load_words<uint8_t, V>(cv, n);
+    const auto wp = load_words<T, V>(p, n);
+    const int pm = first_power(scales[0]), pv = second_power(scales[1]);
+    float m[V], v[V], np[V];
+    uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        m[j] = decode_first(bm.byte(j), pm);
+        v[j] = decode_second(bv.byte(j), pv);
+        const float s = step_of(m[j], v[j], wg[j] * f.grad, b, f);
+        np[j] = wp[j] * f.decay - s;
+        top_m = max(top_m, finite_bits(m[j]));
+        top_v = max(top_v, finite_bits(v[j]));
     }
-    for (int d = 8; d > 0; d >>= 1) {
-        top_m = fmaxf(top_m, __shfl_xor(top_m, d));
-        top_v = fmaxf(top_v, __shfl_xor(top_v, d));
+    store_pack<T, V>(p, np, n);
+    const uint32_t xm = block_exponent(largest16(top_m), kFirstFloor), xv = block_exponent(largest16(top_v), kSecondFloor);
+    const int qm = first_power(xm), qv = second_power(xv);
+    Words<uint8_t, V> om = {}, ov = {};
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const uint32_t h = dither((uint32_t)at + j, f.key);
+        om.w[j / 4] |= encode_first(m[j], qm, (h >> 12 & 0xffff0u) + 8u) << (j % 4 * 8);
+        ov.w[j / 4] |= encode_second(v[j], qv, (h << 4 & 0xffff0u) + 8u) << (j % 4 * 8);
     }
-    if (!live) return;
-    const uint32_t xm = block_exponent(top_m, kFirstFloor), xv = block_exponent(top_v, kSecondFloor);
-    const float sm = power_of_two(kFirstBias - (int)xm), sv = power_of_two(kSecondBias - (int)xv);
-    for (int j = 0; j < 8; ++j) {
-        const int64_t i = i0 + j;
-        if (i >= e.numel) break;
-        const uint32_t h = dither((uint32_t)i, f.key);
-        cm[i] = (uint8_t)encode_first(m[j], sm, h >> 16);
-        cv[i] = (uint8_t)encode_second(v[j], sv, h & 0xffffu);
-    }
+    store_words<uint8_t, V>(cm, om, n);
+    store_words<uint8_t, V>(cv, ov, n);
     if ((threadIdx.x & 15) == 0) {
-        e.scales[2 * block] = (uint8_t)xm;
-        e.scales[2 * block + 1] = (uint8_t)xv;
+        scales[0] = (uint8_t)xm;
+        scales[1] = (uint8_t)xv;
     }
 }
 
+// eight elements per thread, so that a thread's all belong to one block
 __global__ __launch_bounds__(kThreads) void moment_values_kernel(const uint8_t *__restrict__ cm, const uint8_t *__restrict__ cv,
                                                                  const uint8_t *__restrict__ scales, int64_t numel,
                                                                  bf16 *__restrict__ m, bf16 *__restrict__ v)
 {
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < numel; i += (int64_t)gridDim.x * kThreads) {
+    constexpr int V = 8;
+    const int64_t step = (int64_t)gridDim.x * kThreads * V;
+    for (int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * V; i < numel; i += step) {
+        const int n = (int)min(numel - i, (int64_t)V);
+        const auto bm = load_words<uint8_t, V>(cm + i, n), bv = load_words<uint8_t, V>(cv + i, n);
         const int64_t block = i / kBlock;
-        m[i] = from_float<bf16>(decode_first(cm[i], first_unit(scales[2 * block])));
-        v[i] = from_float<bf16>(decode_second(cv[i], second_unit(scales[2 * block + 1])));
+        const int pm = first_power(scales[2 * block]), pv = second_power(scales[2 * block + 1]);
+        float om[V], ov[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            om[j] = decode_first(bm.byte(j), pm);
+            ov[j] = decode_second(bv.byte(j), pv);
+        }
+        store_pack<bf16, V>(m + i, om, n);
+        store_pack<bf16, V>(v + i, ov, n);
     }
 }
 
@@ -453,7 +500,7 @@ extern "C" int sv3d_moment_values(const uint8_t *exp_avg, const uint8_t *exp_avg
     if (numel == 0) return SV3D_OK;
     if (!exp_avg || !exp_avg_sq || !scales || !exp_avg_out || !exp_avg_sq_out || !aligned(exp_avg_out, 2) || !aligned(exp_avg_sq_out, 2))
         return SV3D_ERR_INVALID_ARG;
-    const int64_t groups = (numel + kThreads - 1) / kThreads;
+    const int64_t groups = (numel + kThreads * 8 - 1) / (kThreads * 8);
     hipLaunchKernelGGL(moment_values_kernel, dim3((uint32_t)(groups < (1 << 20) ? groups : (1 << 20))), dim3(kThreads), 0,
                        (hipStream_t)stream, exp_avg, exp_avg_sq, scales, numel, (bf16 *)exp_avg_out, (bf16 *)exp_avg_sq_out);
     return launch_status();

@@ -30,6 +30,7 @@ template <class T, int N>
 struct Words {
     static constexpr int kCount = N * (int)sizeof(T) / 4;
     uint32_t w[kCount];
+    __device__ inline uint32_t byte(int i) const { return w[i / 4] >> (i % 4 * 8) & 0xffu; }
     __device__ inline float operator[](int i) const
     {
         if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
@@ -38,6 +39,11 @@ struct Words {
         return (float)__builtin_bit_cast(f16, (uint16_t)(i & 1 ? h >> 16 : h & 0xffffu));
     }
 };
+
+template <int BYTES> struct Bits;
+template <> struct Bits<1> { using type = uint8_t; };
+template <> struct Bits<2> { using type = uint16_t; };
+template <> struct Bits<4> { using type = uint32_t; };
 
 // `n` of the elements exist (n <= 0: none), the others are zero
 template <class T, int N>
@@ -52,15 +58,40 @@ __device__ inline Words<T, N> load_words(const T *p, int n)
 #pragma unroll
     for (int i = 0; i < r.kCount; ++i) r.w[i] = 0u;
     if (n <= 0) return r;
+    constexpr int kBytes = (int)sizeof(T);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        if (j >= n) break;
-        if constexpr (sizeof(T) == 4)
-            r.w[j] = reinterpret_cast<const uint32_t *>(p)[j];
-        else
-            r.w[j / 2] |= (uint32_t) reinterpret_cast<const uint16_t *>(p)[j] << (j % 2 * 16);
-    }
+    for (int j = 0; j < N; ++j)
+        if (j < n)
+            r.w[j * kBytes / 4] |= (uint32_t) reinterpret_cast<const typename Bits<kBytes>::type *>(p)[j] << (j * kBytes % 4 * 8);
     return r;
+}
+
+// the first n of the elements, all of them at once where they are there
+template <class T, int N>
+__device__ inline void store_words(T *p, const Words<T, N> &r, int n)
+{
+    if (n >= N) {
+        Pack<T, N> q;
+        __builtin_memcpy(q.v, r.w, sizeof(r.w));
+        *reinterpret_cast<Pack<T, N> *>(p) = q;
+        return;
+    }
+    using B = typename Bits<(int)sizeof(T)>::type;
+    constexpr int kBytes = (int)sizeof(T);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        if (j < n) reinterpret_cast<B *>(p)[j] = (B)(r.w[j * kBytes / 4] >> (j * kBytes % 4 * 8));
+}
+
+template <class T, int V>
+__device__ inline void store_pack(T *p, const float *v, int n)
+{
+    Pack<T, V> r;
+#pragma unroll
+    for (int j = 0; j < V; ++j) r.v[j] = from_float<T>(v[j]);
+    Words<T, V> w;
+    __builtin_memcpy(w.w, r.v, sizeof(w.w));
+    store_words<T, V>(p, w, n);
 }
 
 // ---- sums over the lanes of a wave ----------------------------------------------------------------

@@ -36,21 +36,6 @@ __device__ inline float row_sum(float v, float *part)
     return v;
 }
 
-template <class T, int V>
-__device__ inline void store_pack(T *p, const float *v, int n)
-{
-    Pack<T, V> r;
-#pragma unroll
-    for (int j = 0; j < V; ++j) r.v[j] = from_float<T>(v[j]);
-    if (n >= V) {
-        *reinterpret_cast<Pack<T, V> *>(p) = r;
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-        if (j < n) p[j] = r.v[j];
-}
-
 // weights of either type, kept in registers over all the rows of a thread
 template <class X, int V>
 __device__ inline void load_params(const void *p, bool f32, float missing, int c, int n, float *out)
