@@ -393,7 +393,7 @@ int sv3d_grad_square_sums(const sv3d_adamw_tensor *tensors, int32_t num_tensors,
  *   g  = grad / S * min(1, max_norm / (G + 1e-6))       (no factor if square_sums is NULL)
  *   t  = step + 1;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   param = param (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
- * in fp32; the weight is rounded to its type to nearest, 8-bit moments are rounded up or down with the
+ * in fp32 (an eps below 2^-63 counts as 2^-63); the weight is rounded to its type to nearest, 8-bit moments are rounded up or down with the
  * probability of what is cut off, decided by a hash of (element, t, seed), and a positive exp_avg_sq
  * never becomes zero.  `maximize` negates g.  If *found_inf is not 0 nothing is changed.  lr is read from
  * `lr_device` where that is not NULL.  *total_norm (may be NULL) receives G.

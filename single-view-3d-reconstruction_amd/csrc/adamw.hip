@@ -7,27 +7,34 @@
 
 #include <type_traits>
 
+// fused products and sums are written out: the same bits wherever a function is inlined
+#pragma clang fp contract(off)
+
 namespace {
 
 using namespace sv3d;
 
 constexpr int kThreads = 256;
-constexpr int kTable = 64;          // tensors of one launch: the table has to fit 4 KB of kernel arguments
-constexpr int kChunk = 2048;        // elements of one workgroup of the update
+// tensors of one launch: the tables have to fit 4 KB of kernel arguments
+constexpr int kTable = 76;
+constexpr int kSumTable = 250;
+constexpr int64_t kPiece = (int64_t)1 << 31;    // elements of one table entry at most
+constexpr int kChunk = 2048;        // elements of one workgroup of the update, 32-bit moments
+constexpr int kChunk8 = 2048;       // 8-bit moments
 constexpr int kBlock = SV3D_STATE_BLOCK;
 constexpr int kSumChunk = 4096;
 constexpr int kSumGroups = 1024;
-constexpr float kSmallest = 0x1p-126f;
 
 // ---- the norm: sums of squares --------------------------------------------------------------------
 // Squares and sums in double: a square of an fp32 number neither overflows nor is rounded there, and the order of
 // the sum stops to matter for the fp32 norm that is made of it.
 struct SumTable {
-    const void *grad[kTable];
-    int64_t numel[kTable];
-    int32_t first[kTable + 1];      // of each tensor's chunks
+    const void *grad[kSumTable];
+    uint32_t numel[kSumTable];
+    int32_t first[kSumTable + 1];   // of each tensor's chunks
     int32_t count;
 };
+static_assert(sizeof(SumTable) + 8 <= 4096, "kernel arguments");
 
 template <class T>
 __global__ __launch_bounds__(kThreads) void grad_square_sums_kernel(SumTable t, double *__restrict__ sums)
@@ -39,15 +46,24 @@ __global__ __launch_bounds__(kThreads) void grad_square_sums_kernel(SumTable t, 
         while (chunk >= t.first[k + 1]) ++k;
         const T *g = (const T *)t.grad[k];
         const int64_t at = (int64_t)(chunk - t.first[k]) * kSumChunk;
-        const int left = (int)min(t.numel[k] - at, (int64_t)kSumChunk);
-        constexpr int V = 16 / (int)sizeof(T);
+        const int64_t left = (int64_t)t.numel[k] - at;
+        constexpr int V = 16 / (int)sizeof(T), U = kSumChunk / (kThreads * V);
+        Words<T, V> w[U];
+        // a whole chunk's loads go out together; with the ends checked they would wait for each other
+        if (left >= kSumChunk) {
 #pragma unroll
-        for (int u = 0; u < kSumChunk / (kThreads * V); ++u) {
-            const int o = (u * kThreads + threadIdx.x) * V;
-            const auto w = load_words<T, V>(g + at + o, left - o);
+            for (int u = 0; u < U; ++u) w[u] = load_words<T, V>(g + at + (u * kThreads + threadIdx.x) * V);
+        } else {
 #pragma unroll
-            for (int j = 0; j < V; ++j) acc[j & 3] += (double)w[j] * (double)w[j];
+            for (int u = 0; u < U; ++u) {
+                const int o = (u * kThreads + threadIdx.x) * V;
+                w[u] = load_words<T, V>(g + at + o, (int)left - o);
+            }
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j & 3] += (double)w[u][j] * (double)w[u][j];
     }
     double sum = (acc[0] + acc[1]) + (acc[2] + acc[3]);
     for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
@@ -127,48 +143,80 @@ __device__ inline uint32_t dither(uint32_t element, uint32_t key)
     return x ^ (x >> 16);
 }
 
+// First moments are the e4m3 numbers that the hardware converts, rounding included: it adds 20 bits below the last kept one
+// and cuts (here the 16 bits of the dither and half a one).  They are scaled so that a block's largest value lands in
+// [2^7, 2^8).
+//
+// A code of a second moment is the upper bits of a float32 whose exponent field is as narrow as the code's: with the
+// block's values scaled so that the code's smallest exponent meets float32's, bits 20 and up of a value ARE its code, its
+// subnormal codes included (float32's own subnormal numbers), and the same 20 bits go in below before they are cut off.
+// The block's largest value has code 0xf0 to 0xf8.
+constexpr int kFirstBias = 134, kSecondBias = 30;
+constexpr int kFirstFloor = 20, kSecondFloor = 34;      // so that every value is a normal number, also as bf16
+
 __device__ inline float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// A code is the upper bits of a float32 whose exponent field is as narrow as the code's: with a block's values scaled so
-// that the code's smallest exponent meets float32's, bits 20 and up of a value ARE its code, its subnormal codes included
-// (float32's own subnormal numbers), and the dither (16 bits and half a one) goes in below before they are cut off.
-//   first:  field = exponent + 7,  sign in bit 31;     second: field = exponent + 15
-constexpr int kFirstBias = 134, kSecondBias = 142;      // a block's largest value lands in [2^7, 2^8) and [2^15, 2^16)
-constexpr int kFirstFloor = 20, kSecondFloor = 34;      // so that every value is a normal number, also as bf16
-constexpr int kFirstField = 127 - 7, kSecondField = 127 - 15;
-
-// what to multiply by two to the power of, from a value to its code's place; a byte below the lowest that is ever
-// written (fresh state: 0) counts as that one
-__device__ inline int first_power(uint32_t e) { return kFirstBias - kFirstField - max((int)e, kFirstFloor); }
-__device__ inline int second_power(uint32_t e) { return kSecondBias - kSecondField - max((int)e, kSecondFloor); }
-
-__device__ inline uint32_t block_exponent(uint32_t largest_bits, int floor) { return (uint32_t)max((int)(largest_bits >> 23), floor); }
+// a byte below the lowest that is ever written (fresh state: 0) counts as that one
+__device__ inline float first_unit(uint32_t e) { return power_of_two(max((int)e, kFirstFloor) - kFirstBias); }
+__device__ inline int second_power(uint32_t e) { return max((int)e, kSecondFloor) - kSecondBias; }
 
 constexpr uint32_t kInfinity = 0x7f800000u;
 __device__ inline uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 // what a moment contributes to its block's exponent: an infinity or NaN does not
 __device__ inline uint32_t finite_bits(float v) { return magnitude_bits(v) < kInfinity ? magnitude_bits(v) : 0u; }
 
-// `low`: the dither bits in place, (bits << 4) + 8
-__device__ inline uint32_t encode_first(float m, int power, uint32_t low)
+// four codes of one word
+__device__ inline void decode_first(uint32_t codes, float unit, float *out)
 {
-    const uint32_t q = (__float_as_uint(ldexpf(m, power)) + low) >> 20;
-    return (magnitude_bits(m) < kInfinity ? q & 0x7fu : 0x7fu) | (q >> 4 & 0x80u);
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+    out[0] = lo[0] * unit;
+    out[1] = lo[1] * unit;
+    out[2] = hi[0] * unit;
+    out[3] = hi[1] * unit;
 }
 
-__device__ inline uint32_t encode_second(float v, int power, uint32_t low)
+__device__ inline void decode_second(uint32_t codes, int power, float *out)
 {
-    const uint32_t q = (__float_as_uint(ldexpf(v, power)) + low) >> 20;
-    return !(v < INFINITY) ? 0xffu : v > 0.f ? max(q, 1u) : q;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = ldexpf(__uint_as_float((codes >> (8 * j) & 0xffu) << 20), power);
+    // 0xff is no number: the only byte whose low seven bits and one carry into its top bit, and whose top bit is set
+    const uint32_t nan = ((codes & 0x7f7f7f7fu) + 0x01010101u) & codes & 0x80808080u;
+    if (nan) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (nan >> (8 * j) & 0xffu) out[j] = NAN;
+    }
 }
 
-__device__ inline float decode_first(uint32_t code, int power)
+// four values, all of them finite, to one word; `h` their dithers
+__device__ inline uint32_t encode_first(const float *m, float scale, const uint32_t *h)
 {
-    const float v = ldexpf(__uint_as_float((code & 0x7fu) << 20 | (code & 0x80u) << 24), -power);
-    return (code & 0x7fu) == 0x7fu ? NAN : v;
+    int w = 0;
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(m[0] * scale, (int)((h[0] & 0xffff0000u) | 0x8000u), w, 0);
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(m[1] * scale, (int)((h[1] & 0xffff0000u) | 0x8000u), w, 1);
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(m[2] * scale, (int)((h[2] & 0xffff0000u) | 0x8000u), w, 2);
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(m[3] * scale, (int)((h[3] & 0xffff0000u) | 0x8000u), w, 3);
+    return (uint32_t)w;
 }
 
-__device__ inline float decode_second(uint32_t code, int power) { return code == 0xffu ? NAN : ldexpf(__uint_as_float(code << 20), -power); }
+__device__ inline uint32_t encode_second(const float *v, int power, const uint32_t *h)
+{
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t q = (__float_as_uint(ldexpf(v[j], -power)) + ((h[j] & 0xffffu) << 4) + 8u) >> 20 & 0xffu;
+        w |= max(q, min(__float_as_uint(v[j]), 1u)) << (8 * j);         // nothing above zero becomes zero
+    }
+    return w;
+}
+
+// in place of the codes that the above made of infinities and NaN
+__device__ inline void mark_not_finite(const float *v, uint32_t code, uint32_t *w)
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (magnitude_bits(v[j]) >= kInfinity) *w = (*w & ~(0xffu << (8 * j))) | (code | (code == 0x7fu ? __float_as_uint(v[j]) >> 31 << 7 : 0u)) << (8 * j);
+}
 
 // ---- the update --------------------------------------------------------------------------------------
 struct Entry {
@@ -176,60 +224,77 @@ struct Entry {
     const void *grad;
     void *exp_avg, *exp_avg_sq;
     uint8_t *scales;
-    int64_t numel;
 };
 
 struct Table {
     Entry t[kTable];
+    uint32_t numel[kTable];
     int32_t first[kTable + 1];
     int32_t order[kTable];              // whose factors
+    uint8_t odd[kTable];                // whether the piece starts at an odd multiple of 2^31 elements
     int32_t count;
 };
 
 struct Betas {
     float b1, c1, b2, c2, eps;          // c = 1 - b, taken in double
 };
+static_assert(sizeof(Table) + sizeof(Betas) + 16 <= 4096, "kernel arguments");
 
-// Products and sums of the moments as they stand, each rounded: the same bits on every path.  The root and the
-// quotient are the hardware's (off by one unit in the last place where the exact ones are off by half); it takes numbers
-// below the normal ones for zero, hence the lower end.
-__device__ inline float step_of(float &m, float &v, float g, const Betas &b, const Factors &f)
+// New moments and weight.  The root and the quotient are the hardware's: off by one unit in the last place where the exact
+// ones are off by half.  Its root takes numbers below the normal ones (2^-126) for zero; eps is at least 2^-63, the root
+// of that.
+__device__ inline float step_of(float p, float &m, float &v, float g, const Betas &b, const Factors &f)
 {
-    m = __fadd_rn(__fmul_rn(b.b1, m), __fmul_rn(b.c1, g));
-    v = __fadd_rn(__fmul_rn(b.b2, v), __fmul_rn(b.c2, __fmul_rn(g, g)));
-    const float root = __builtin_amdgcn_sqrtf(v < kSmallest ? kSmallest : v);       // NaN stays
-    return f.rate * (m * __builtin_amdgcn_rcpf(root * f.root + b.eps));
+    g *= f.grad;
+    m = fmaf(b.c1, g, b.b1 * m);
+    v = fmaf(b.c2 * g, g, b.b2 * v);
+    const float u = m * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_sqrtf(v), f.root, b.eps));
+    return fmaf(-f.rate, u, p * f.decay);
 }
 
-// The tensor of chunk `chunk`: the lanes look at the 64 table entries at once.
+// The tensor of chunk `chunk`: the lanes look at the table's entries at once, two each.
 __device__ inline int tensor_of(const int32_t *first, int count, int chunk)
 {
+    static_assert(kTable > 64 && kTable <= 128, "two entries per lane");
     const int lane = threadIdx.x & 63;
-    return __popcll(__ballot(lane < count && chunk >= first[lane + 1]));
+    return __popcll(__ballot(lane < count && chunk >= first[lane + 1])) +
+           __popcll(__ballot(lane + 64 < count && chunk >= first[min(lane + 65, kTable)]));
 }
 
-template <class T>
-__global__ __launch_bounds__(kThreads) void adamw_kernel(Table t, Betas b, const Factors *__restrict__ factors)
+// A whole chunk's loads go out together; with the ends checked they would wait for each other, which only a tensor's last
+// chunk does.
+template <bool WHOLE, class T, int V>
+__device__ inline Words<T, V> load_some(const T *p, int n)
 {
-    const int k = __builtin_amdgcn_readfirstlane(tensor_of(t.first, t.count, blockIdx.x));
-    const Entry e = t.t[k];
-    const Factors f = factors[t.order[k]];
-    if (f.skip) return;
+    if constexpr (WHOLE) return load_words<T, V>(p);
+    return load_words<T, V>(p, n);
+}
+
+template <bool WHOLE, class T, int V>
+__device__ inline void store_some(T *p, const Words<T, V> &w, int n)
+{
+    if constexpr (WHOLE)
+        store_words<T, V>(p, w);
+    else
+        store_words<T, V>(p, w, n);
+}
+
+template <bool WHOLE, class T>
+__device__ inline void update_chunk(const Entry &e, int64_t at, int left, const Betas &b, const Factors &f)
+{
     constexpr int V = 4, U = kChunk / (kThreads * V);
-    const int64_t at = (int64_t)((int)blockIdx.x - t.first[k]) * kChunk + threadIdx.x * V;
     T *p = (T *)e.param + at;
     const T *g = (const T *)e.grad + at;
     float *em = (float *)e.exp_avg + at, *ev = (float *)e.exp_avg_sq + at;
-    const int left = (int)min(e.numel - at, (int64_t)kChunk);
     Words<T, V> wp[U], wg[U];
     Words<float, V> wm[U], wv[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int o = u * kThreads * V, n = left - o;
-        wg[u] = load_words<T, V>(g + o, n);
-        wm[u] = load_words<float, V>(em + o, n);
-        wv[u] = load_words<float, V>(ev + o, n);
-        wp[u] = load_words<T, V>(p + o, n);
+        wg[u] = load_some<WHOLE, T, V>(g + o, n);
+        wm[u] = load_some<WHOLE, float, V>(em + o, n);
+        wv[u] = load_some<WHOLE, float, V>(ev + o, n);
+        wp[u] = load_some<WHOLE, T, V>(p + o, n);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -239,13 +304,26 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(Table t, Betas b, const
         for (int j = 0; j < V; ++j) {
             nm[j] = wm[u][j];
             nv[j] = wv[u][j];
-            const float s = step_of(nm[j], nv[j], wg[u][j] * f.grad, b, f);
-            np[j] = wp[u][j] * f.decay - s;
+            np[j] = step_of(wp[u][j], nm[j], nv[j], wg[u][j], b, f);
         }
-        store_pack<float, V>(em + o, nm, n);
-        store_pack<float, V>(ev + o, nv, n);
-        store_pack<T, V>(p + o, np, n);
+        store_some<WHOLE, float, V>(em + o, to_words<float, V>(nm), n);
+        store_some<WHOLE, float, V>(ev + o, to_words<float, V>(nv), n);
+        store_some<WHOLE, T, V>(p + o, to_words<T, V>(np), n);
     }
+}
+
+template <class T>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(Table t, Betas b, const Factors *__restrict__ factors)
+{
+    const int chunk = blockIdx.x, k = __builtin_amdgcn_readfirstlane(tensor_of(t.first, t.count, chunk));
+    const Factors f = factors[t.order[k]];
+    if (f.skip) return;
+    const int64_t from = (int64_t)(chunk - t.first[k]) * kChunk, left = (int64_t)t.numel[k] - from;
+    const int mine = threadIdx.x * 4;
+    if (left >= kChunk)
+        update_chunk<true, T>(t.t[k], from + mine, 0, b, f);
+    else
+        update_chunk<false, T>(t.t[k], from + mine, (int)left - mine, b, f);
 }
 
 // the largest of 16 neighbouring lanes, in each of them
@@ -259,52 +337,86 @@ __device__ inline uint32_t largest16(uint32_t v)
 
 // 16 lanes share a block of 128 elements, eight each.  Elements behind the end are zero: they add nothing to the
 // block's exponents and are not stored.
-template <class T>
-__global__ __launch_bounds__(kThreads) void adamw8_kernel(Table t, Betas b, const Factors *__restrict__ factors)
+template <bool WHOLE, class T>
+__device__ inline void update_chunk8(const Entry &e, int64_t at, int n, uint32_t element, const Betas &b, const Factors &f)
 {
-    const int k = __builtin_amdgcn_readfirstlane(tensor_of(t.first, t.count, blockIdx.x));
-    const Entry e = t.t[k];
-    const Factors f = factors[t.order[k]];
-    if (f.skip) return;
     constexpr int V = 8;
-    const int64_t at = (int64_t)((int)blockIdx.x - t.first[k]) * kChunk + threadIdx.x * V;
-    // the 16 lanes of a block stay or go together: each of them passes on what others found
-    if (at - (int)(threadIdx.x & 15) * V >= e.numel) return;
-    const int n = (int)max(min(e.numel - at, (int64_t)V), (int64_t)0);
     T *p = (T *)e.param + at;
     const T *g = (const T *)e.grad + at;
     uint8_t *cm = (uint8_t *)e.exp_avg + at, *cv = (uint8_t *)e.exp_avg_sq + at;
     uint8_t *scales = e.scales + at / kBlock * 2;
-    const auto wg = load_words<T, V>(g, n);
-    const auto bm = load_words<uint8_t, V>(cm, n), bv = load_words<uint8_t, V>(cv, n);
-    const auto wp = load_words<T, V>(p, n);
-    const int pm = first_power(scales[0]), pv = second_power(scales[1]);
+    const auto bm = load_some<WHOLE, uint8_t, V>(cm, n), bv = load_some<WHOLE, uint8_t, V>(cv, n);
+    const uint32_t em = scales[0], ev = scales[1];
+    const auto wg = load_some<WHOLE, T, V>(g, n), wp = load_some<WHOLE, T, V>(p, n);
     float m[V], v[V], np[V];
+    const float unit = first_unit(em);
+    const int power = second_power(ev);
+#pragma unroll
+    for (int q = 0; q < V; q += 4) {
+        decode_first(bm.w[q / 4], unit, m + q);
+        decode_second(bv.w[q / 4], power, v + q);
+    }
     uint32_t top_m = 0, top_v = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        m[j] = decode_first(bm.byte(j), pm);
-        v[j] = decode_second(bv.byte(j), pv);
-        const float s = step_of(m[j], v[j], wg[j] * f.grad, b, f);
-        np[j] = wp[j] * f.decay - s;
-        top_m = max(top_m, finite_bits(m[j]));
-        top_v = max(top_v, finite_bits(v[j]));
+        np[j] = step_of(wp[j], m[j], v[j], wg[j], b, f);
+        top_m = max(top_m, magnitude_bits(m[j]));
+        top_v = max(top_v, magnitude_bits(v[j]));
     }
-    store_pack<T, V>(p, np, n);
-    const uint32_t xm = block_exponent(largest16(top_m), kFirstFloor), xv = block_exponent(largest16(top_v), kSecondFloor);
-    const int qm = first_power(xm), qv = second_power(xv);
-    Words<uint8_t, V> om = {}, ov = {};
+    store_some<WHOLE, T, V>(p, to_words<T, V>(np), n);
+    top_m = largest16(top_m);
+    top_v = largest16(top_v);
+    const bool wild = max(top_m, top_v) >= kInfinity;       // the same in the block's 16 lanes
+    if (wild) {
+        top_m = top_v = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const uint32_t h = dither((uint32_t)at + j, f.key);
-        om.w[j / 4] |= encode_first(m[j], qm, (h >> 12 & 0xffff0u) + 8u) << (j % 4 * 8);
-        ov.w[j / 4] |= encode_second(v[j], qv, (h << 4 & 0xffff0u) + 8u) << (j % 4 * 8);
+        for (int j = 0; j < V; ++j) {
+            top_m = max(top_m, finite_bits(m[j]));
+            top_v = max(top_v, finite_bits(v[j]));
+        }
+        top_m = largest16(top_m);
+        top_v = largest16(top_v);
     }
-    store_words<uint8_t, V>(cm, om, n);
-    store_words<uint8_t, V>(cv, ov, n);
+    const int xm = max((int)(top_m >> 23), kFirstFloor), xv = max((int)(top_v >> 23), kSecondFloor);
+    uint32_t h[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) h[j] = dither(element + j, f.key);
+    Words<uint8_t, V> om, ov;
+#pragma unroll
+    for (int q = 0; q < V; q += 4) {
+        om.w[q / 4] = encode_first(m + q, power_of_two(kFirstBias - xm), h + q);
+        ov.w[q / 4] = encode_second(v + q, second_power(xv), h + q);
+    }
+    if (wild) {
+#pragma unroll
+        for (int q = 0; q < V; q += 4) {
+            mark_not_finite(m + q, 0x7fu, &om.w[q / 4]);
+            mark_not_finite(v + q, 0xffu, &ov.w[q / 4]);
+        }
+    }
+    store_some<WHOLE, uint8_t, V>(cm, om, n);
+    store_some<WHOLE, uint8_t, V>(cv, ov, n);
     if ((threadIdx.x & 15) == 0) {
         scales[0] = (uint8_t)xm;
         scales[1] = (uint8_t)xv;
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(kThreads) void adamw8_kernel(Table t, Betas b, const Factors *__restrict__ factors)
+{
+    const int chunk = blockIdx.x, k = __builtin_amdgcn_readfirstlane(tensor_of(t.first, t.count, chunk));
+    const Factors f = factors[t.order[k]];
+    if (f.skip) return;
+    const int64_t from = (int64_t)(chunk - t.first[k]) * kChunk8, left = (int64_t)t.numel[k] - from;
+    const int mine = threadIdx.x * 8;
+    const uint32_t element = (uint32_t)from + mine + ((uint32_t)t.odd[k] << 31);
+    if (left >= kChunk8) {
+        update_chunk8<true, T>(t.t[k], from + mine, 0, element, b, f);
+    } else {
+        // the 16 lanes of a block stay or go together: each of them passes on what others found
+        if (mine / kBlock * kBlock >= left) return;
+        update_chunk8<false, T>(t.t[k], from + mine, (int)left - mine, element, b, f);
     }
 }
 
@@ -319,12 +431,13 @@ __global__ __launch_bounds__(kThreads) void moment_values_kernel(const uint8_t *
         const int n = (int)min(numel - i, (int64_t)V);
         const auto bm = load_words<uint8_t, V>(cm + i, n), bv = load_words<uint8_t, V>(cv + i, n);
         const int64_t block = i / kBlock;
-        const int pm = first_power(scales[2 * block]), pv = second_power(scales[2 * block + 1]);
+        const float unit = first_unit(scales[2 * block]);
+        const int power = second_power(scales[2 * block + 1]);
         float om[V], ov[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            om[j] = decode_first(bm.byte(j), pm);
-            ov[j] = decode_second(bv.byte(j), pv);
+        for (int q = 0; q < V; q += 4) {
+            decode_first(bm.w[q / 4], unit, om + q);
+            decode_second(bv.w[q / 4], power, ov + q);
         }
         store_pack<bf16, V>(m + i, om, n);
         store_pack<bf16, V>(v + i, ov, n);
@@ -349,29 +462,29 @@ int check(const sv3d_adamw_tensor *tensors, int32_t n, bool grads_only)
     return SV3D_OK;
 }
 
-// Collects tensors into launches of at most kTable of them and kMaxChunks chunks (a launch holds fewer than 2^32
-// threads) and calls launch(pieces, first chunk of each, number of pieces).  Only a tensor that is larger than a
-// launch is cut, at multiples of kMaxChunks chunks.
+// Collects tensors into launches of at most TABLE pieces and kMaxChunks chunks (a launch holds fewer than 2^32
+// threads) and calls launch(pieces, first chunk of each, number of pieces).  A tensor of more than kPiece elements is
+// several pieces.
 constexpr int64_t kMaxChunks = 1 << 23;
-static_assert(kMaxChunks * kChunk % ((int64_t)1 << 32) == 0, "the dither takes an element's index modulo 2^32");
+static_assert(kPiece / kChunk <= kMaxChunks && kPiece % kChunk == 0 && kPiece % kChunk8 == 0 && kPiece % kSumChunk == 0, "a piece fits a launch");
 
 struct Piece {
     int32_t index;
     int64_t from, numel;
 };
 
-template <class Take, class Launch>
+template <int TABLE, class Take, class Launch>
 int in_launches(const sv3d_adamw_tensor *tensors, int32_t n, int64_t chunk, Take take, Launch launch)
 {
-    Piece piece[kTable];
-    int32_t first[kTable + 1] = {0};
+    Piece piece[TABLE];
+    int32_t first[TABLE + 1] = {0};
     int count = 0;
     for (int32_t i = 0; i < n; ++i) {
         if (!take(tensors[i])) continue;
-        for (int64_t from = 0; from < tensors[i].numel; from += kMaxChunks * chunk) {
-            const int64_t left = tensors[i].numel - from, most = kMaxChunks * chunk;
-            const int64_t now = left < most ? left : most, chunks = (now + chunk - 1) / chunk;
-            if (count == kTable || first[count] + chunks > kMaxChunks) {
+        for (int64_t from = 0; from < tensors[i].numel; from += kPiece) {
+            const int64_t left = tensors[i].numel - from, now = left < kPiece ? left : kPiece;
+            const int64_t chunks = (now + chunk - 1) / chunk;
+            if (count == TABLE || first[count] + chunks > kMaxChunks) {
                 if (const int st = launch(piece, first, count)) return st;
                 count = 0;
             }
@@ -401,7 +514,7 @@ extern "C" int sv3d_grad_square_sums_count(const sv3d_adamw_tensor *tensors, int
     if (const int st = check(tensors, num_tensors, true)) return st;
     int32_t total = 0;
     for_each_type([&](auto *, int32_t type) {
-        return in_launches(tensors, num_tensors, kSumChunk, [&](const sv3d_adamw_tensor &t) { return t.type == type; },
+        return in_launches<kSumTable>(tensors, num_tensors, kSumChunk, [&](const sv3d_adamw_tensor &t) { return t.type == type; },
                            [&](const Piece *, const int32_t *first, int n) {
                                total += sum_groups(first[n]);
                                return (int)SV3D_OK;
@@ -419,13 +532,13 @@ extern "C" int sv3d_grad_square_sums(const sv3d_adamw_tensor *tensors, int32_t n
     if (count != need || (need > 0 && (!sums || !aligned(sums, 8)))) return SV3D_ERR_INVALID_ARG;
     return for_each_type([&](auto *T, int32_t type) {
         using E = std::remove_pointer_t<decltype(T)>;
-        return in_launches(tensors, num_tensors, kSumChunk, [&](const sv3d_adamw_tensor &t) { return t.type == type; },
+        return in_launches<kSumTable>(tensors, num_tensors, kSumChunk, [&](const sv3d_adamw_tensor &t) { return t.type == type; },
                            [&](const Piece *piece, const int32_t *first, int n) {
                                SumTable t;
                                t.count = n;
                                for (int k = 0; k < n; ++k) {
                                    t.grad[k] = (const E *)tensors[piece[k].index].grad + piece[k].from;
-                                   t.numel[k] = piece[k].numel;
+                                   t.numel[k] = (uint32_t)piece[k].numel;
                                }
                                for (int k = 0; k <= n; ++k) t.first[k] = first[k];
                                const int groups = sum_groups(first[n]);
@@ -463,13 +576,14 @@ extern "C" int sv3d_adamw_step(const sv3d_adamw_params *p, const sv3d_adamw_tens
         hipLaunchKernelGGL(adamw_factors_kernel, dim3(1), dim3(kThreads), 0, (hipStream_t)stream, s, *p, factors);
         if (const int st = launch_status()) return st;
     }
-    const Betas b = {(float)p->beta1, (float)(1.0 - p->beta1), (float)p->beta2, (float)(1.0 - p->beta2), (float)p->eps};
+    const Betas b = {(float)p->beta1, (float)(1.0 - p->beta1), (float)p->beta2, (float)(1.0 - p->beta2),
+                     (float)(p->eps > 0x1p-63 ? p->eps : 0x1p-63)};
     return for_each_type([&](auto *T, int32_t type) {
         using E = std::remove_pointer_t<decltype(T)>;
         for (int32_t bits : {32, 8}) {
             const int64_t state = bits == 32 ? 4 : 1;
-            const int st = in_launches(
-                tensors, num_tensors, kChunk,
+            const int st = in_launches<kTable>(
+                tensors, num_tensors, bits == 32 ? kChunk : kChunk8,
                 [&](const sv3d_adamw_tensor &t) { return t.type == type && t.state_bits == bits; },
                 [&](const Piece *piece, const int32_t *first, int n) {
                     Table t;
@@ -478,9 +592,10 @@ extern "C" int sv3d_adamw_step(const sv3d_adamw_params *p, const sv3d_adamw_tens
                         const sv3d_adamw_tensor &s = tensors[piece[k].index];
                         const int64_t from = piece[k].from;
                         t.t[k] = {(E *)s.param + from, (const E *)s.grad + from, (char *)s.exp_avg + from * state,
-                                  (char *)s.exp_avg_sq + from * state, s.scales ? s.scales + from / kBlock * 2 : nullptr,
-                                  piece[k].numel};
+                                  (char *)s.exp_avg_sq + from * state, s.scales ? s.scales + from / kBlock * 2 : nullptr};
+                        t.numel[k] = (uint32_t)piece[k].numel;
                         t.order[k] = piece[k].index;
+                        t.odd[k] = (uint8_t)(from >> 31 & 1);
                     }
                     for (int k = 0; k <= n; ++k) t.first[k] = first[k];
                     const auto kernel = bits == 32 ? adamw_kernel<E> : adamw8_kernel<E>;

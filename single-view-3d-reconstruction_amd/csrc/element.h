@@ -45,18 +45,30 @@ template <> struct Bits<1> { using type = uint8_t; };
 template <> struct Bits<2> { using type = uint16_t; };
 template <> struct Bits<4> { using type = uint32_t; };
 
+// all of them
+template <class T, int N>
+__device__ inline Words<T, N> load_words(const T *p)
+{
+    Words<T, N> r;
+    const auto q = *reinterpret_cast<const Pack<T, N> *>(p);
+    __builtin_memcpy(r.w, q.v, sizeof(r.w));
+    return r;
+}
+
+template <class T, int N>
+__device__ inline void store_words(T *p, const Words<T, N> &r)
+{
+    Pack<T, N> q;
+    __builtin_memcpy(q.v, r.w, sizeof(r.w));
+    *reinterpret_cast<Pack<T, N> *>(p) = q;
+}
+
 // `n` of the elements exist (n <= 0: none), the others are zero
 template <class T, int N>
 __device__ inline Words<T, N> load_words(const T *p, int n)
 {
-    Words<T, N> r;
-    if (n >= N) {
-        const auto q = *reinterpret_cast<const Pack<T, N> *>(p);
-        __builtin_memcpy(r.w, q.v, sizeof(r.w));
-        return r;
-    }
-#pragma unroll
-    for (int i = 0; i < r.kCount; ++i) r.w[i] = 0u;
+    if (n >= N) return load_words<T, N>(p);
+    Words<T, N> r = {};
     if (n <= 0) return r;
     constexpr int kBytes = (int)sizeof(T);
 #pragma unroll
@@ -70,12 +82,7 @@ __device__ inline Words<T, N> load_words(const T *p, int n)
 template <class T, int N>
 __device__ inline void store_words(T *p, const Words<T, N> &r, int n)
 {
-    if (n >= N) {
-        Pack<T, N> q;
-        __builtin_memcpy(q.v, r.w, sizeof(r.w));
-        *reinterpret_cast<Pack<T, N> *>(p) = q;
-        return;
-    }
+    if (n >= N) return store_words<T, N>(p, r);
     using B = typename Bits<(int)sizeof(T)>::type;
     constexpr int kBytes = (int)sizeof(T);
 #pragma unroll
@@ -84,15 +91,18 @@ __device__ inline void store_words(T *p, const Words<T, N> &r, int n)
 }
 
 template <class T, int V>
-__device__ inline void store_pack(T *p, const float *v, int n)
+__device__ inline Words<T, V> to_words(const float *v)
 {
     Pack<T, V> r;
 #pragma unroll
     for (int j = 0; j < V; ++j) r.v[j] = from_float<T>(v[j]);
     Words<T, V> w;
     __builtin_memcpy(w.w, r.v, sizeof(w.w));
-    store_words<T, V>(p, w, n);
+    return w;
 }
+
+template <class T, int V>
+__device__ inline void store_pack(T *p, const float *v, int n) { store_words<T, V>(p, to_words<T, V>(v), n); }
 
 // ---- sums over the lanes of a wave ----------------------------------------------------------------
 // Every one of G neighbouring lanes gets the sum of their values, added in an order that G fixes.

@@ -504,3 +504,35 @@ def test_operator_registration():
                           test_utils=("test_schema", "test_faketensor"))
     torch.library.opcheck(torch.ops.sv3d.moment_values.default, (s.m[0], s.v[0], s.e[0]), test_utils=("test_schema", "test_faketensor"))
     torch.library.opcheck(torch.ops.sv3d.grad_square_sums.default, (s.g,), test_utils=("test_schema", "test_faketensor"))
+
+
+def test_more_elements_than_32_bits_count():
+    """2^32 + 300 elements: a tensor's pieces start at multiples of 2^31, elements 2^32 apart share their dither."""
+    n, far, mid = 2 ** 32 + 300, 2 ** 32, 2 ** 31
+    small = Set([300], BF16, 8, seed=1)
+    p, g = (torch.zeros(n, dtype=BF16, device="cuda") for _ in range(2))
+    m, v = (torch.zeros(n, dtype=torch.uint8, device="cuda") for _ in range(2))
+    e, step = torch.zeros(-(-n // 128), 2, dtype=torch.uint8, device="cuda"), small.steps[0].clone()
+    for at in (0, mid, far):
+        for big, little in ((p, small.p[0]), (g, small.g[0]), (m, small.m[0]), (v, small.v[0])):
+            big[at: at + 300] = little
+        e[at // 128: at // 128 + 3] = small.e[0]
+    sums = optim.grad_square_sums([g])
+    assert abs(float(sums.sum()) - 3 * float((wide(small.g[0]) ** 2).sum())) < 1e-9
+    before = small.values()[0]
+    optim.adamw_step([p], [g], [m], [v], [step], scales=[e], **HYPER)
+    small.step()
+    for at in (0, far):
+        for big, little in ((p, small.p[0]), (m, small.m[0]), (v, small.v[0])):
+            assert torch.equal(big[at: at + 300], little)
+        assert torch.equal(e[at // 128: at // 128 + 3], small.e[0])
+    assert torch.equal(p[mid: mid + 300], small.p[0])
+    want = to.adamw(*before[:4], 3.0, **HYPER)
+    x = (torch.arange(300) + mid + 4 * 0x9E3779B1) % 2 ** 32
+    x = (x ^ (x >> 16)) * 0x6A09E667 % 2 ** 32
+    x = (x ^ (x >> 15)) * 0xBB67AE85 % 2 ** 32
+    x = x ^ (x >> 16)
+    bytes_mid = e[mid // 128: mid // 128 + 3].cpu()
+    assert_codes(to.decode(m[mid: mid + 300].cpu(), bytes_mid[:, 0], to.FIRST), want["m"], want["e_m"], bytes_mid[:, 0], to.FIRST,
+                 x // 65536, "exp_avg")
+    assert not p[300:1000].any() and not p[mid + 300: mid + 1000].any() and not m[far - 1000: far].any()
