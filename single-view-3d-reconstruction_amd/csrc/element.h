@@ -63,11 +63,36 @@ __device__ inline void store_words(T *p, const Words<T, N> &r)
     *reinterpret_cast<Pack<T, N> *>(p) = q;
 }
 
-// `n` of the elements exist (n <= 0: none), the others are zero
+// the same past the caches, for what nobody reads again soon
 template <class T, int N>
+__device__ inline Words<T, N> stream_words(const T *p)
+{
+    using V = uint32_t __attribute__((ext_vector_type(Words<T, N>::kCount), aligned(sizeof(T))));
+    const V q = __builtin_nontemporal_load(reinterpret_cast<const V *>(p));
+    Words<T, N> r;
+    __builtin_memcpy(r.w, &q, sizeof(r.w));
+    return r;
+}
+
+template <class T, int N>
+__device__ inline void stream_words(T *p, const Words<T, N> &r)
+{
+    using V = uint32_t __attribute__((ext_vector_type(Words<T, N>::kCount), aligned(sizeof(T))));
+    V q;
+    __builtin_memcpy(&q, r.w, sizeof(r.w));
+    __builtin_nontemporal_store(q, reinterpret_cast<V *>(p));
+}
+
+// `n` of the elements exist (n <= 0: none), the others are zero.  Without ENDS it is all or none of them.
+template <class T, int N, bool ENDS = true, bool STREAM = false>
 __device__ inline Words<T, N> load_words(const T *p, int n)
 {
-    if (n >= N) return load_words<T, N>(p);
+    if constexpr (!ENDS) {
+        Words<T, N> r = {};
+        if (n > 0) r = STREAM ? stream_words<T, N>(p) : load_words<T, N>(p);
+        return r;
+    }
+    if (n >= N) return STREAM ? stream_words<T, N>(p) : load_words<T, N>(p);
     Words<T, N> r = {};
     if (n <= 0) return r;
     constexpr int kBytes = (int)sizeof(T);
@@ -78,11 +103,30 @@ __device__ inline Words<T, N> load_words(const T *p, int n)
     return r;
 }
 
-// the first n of the elements, all of them at once where they are there
+// Drops the lowest `off` elements, zeros come in at the top.
 template <class T, int N>
+__device__ inline void drop_words(Words<T, N> &r, int off)
+{
+    constexpr int C = Words<T, N>::kCount;
+    const int bytes = off * (int)sizeof(T);
+#pragma unroll
+    for (int step = C / 2; step > 0; step /= 2)
+        if (bytes & (4 * step)) {
+#pragma unroll
+            for (int i = 0; i < C; ++i) r.w[i] = i + step < C ? r.w[i + step] : 0u;
+        }
+    if (sizeof(T) == 2 && (bytes & 2)) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) r.w[i] = r.w[i] >> 16 | (i + 1 < C ? r.w[i + 1] << 16 : 0u);
+    }
+}
+
+// the first n of the elements, all of them at once where they are there
+template <class T, int N, bool ENDS = true, bool STREAM = false>
 __device__ inline void store_words(T *p, const Words<T, N> &r, int n)
 {
-    if (n >= N) return store_words<T, N>(p, r);
+    if (!ENDS && n <= 0) return;
+    if (!ENDS || n >= N) return STREAM ? stream_words<T, N>(p, r) : store_words<T, N>(p, r);
     using B = typename Bits<(int)sizeof(T)>::type;
     constexpr int kBytes = (int)sizeof(T);
 #pragma unroll
@@ -101,8 +145,8 @@ __device__ inline Words<T, V> to_words(const float *v)
     return w;
 }
 
-template <class T, int V>
-__device__ inline void store_pack(T *p, const float *v, int n) { store_words<T, V>(p, to_words<T, V>(v), n); }
+template <class T, int V, bool ENDS = true, bool STREAM = false>
+__device__ inline void store_pack(T *p, const float *v, int n) { store_words<T, V, ENDS, STREAM>(p, to_words<T, V>(v), n); }
 
 // ---- sums over the lanes of a wave ----------------------------------------------------------------
 // Every one of G neighbouring lanes gets the sum of their values, added in an order that G fixes.

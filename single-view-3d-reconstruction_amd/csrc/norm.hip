@@ -21,6 +21,15 @@ constexpr int kPack = 16 / (int)sizeof(X);
 template <int G>
 constexpr int kGroup = G > 256 ? G : 256;       // threads of the workgroup
 
+// Which of a workgroup's rows a thread works on: known to the whole wave (and kept in scalar registers, the row's
+// addresses with it) where a wave has no more than one.
+template <int G>
+__device__ inline int row_of_group()
+{
+    const int r = threadIdx.x / G;
+    return G >= 64 ? __builtin_amdgcn_readfirstlane(r) : r;
+}
+
 // The sum over the row's threads.  `part` is not written again before every thread has passed another row_sum on
 // another buffer, so one barrier is enough.
 template <int G>
@@ -36,25 +45,47 @@ __device__ inline float row_sum(float v, float *part)
     return v;
 }
 
+// A row's packs.  Where the row's end cuts one, the pack that ends with the row is loaded in its place and what it
+// repeats is dropped when the values are used (drop_end): put together from single elements, a pack would have to
+// be waited for where it is loaded, and no load of the next row would be on its way during the work on this one.  Rows of
+// eight packs at most, which may be shorter than one, are put together.
+template <class X, int G, bool ENDS>
+__device__ inline int cut_by(int n)
+{
+    return ENDS && G > 8 && n > 0 && n < kPack<X> ? kPack<X> - n : 0;
+}
+
+template <class T, int V, int G, bool ENDS>
+__device__ inline Words<T, V> load_row(const T *p, int n, int cut)
+{
+    return load_words<T, V, (ENDS && G <= 8)>(p - cut, n);
+}
+
+template <int G, bool ENDS, class T, int V>
+__device__ inline void drop_end(Words<T, V> &w, int cut)
+{
+    if (ENDS && G > 8 && cut) drop_words(w, cut);
+}
+
 // weights of either type, kept in registers over all the rows of a thread
-template <class X, int V>
+template <class X, int V, bool ENDS>
 __device__ inline void load_params(const void *p, bool f32, float missing, int c, int n, float *out)
 {
     if (!p) {
 #pragma unroll
         for (int j = 0; j < V; ++j) out[j] = missing;
     } else if (f32 || __is_same(X, float)) {
-        const auto r = load_words<float, V>((const float *)p + c, n);
+        const auto r = load_words<float, V, ENDS>((const float *)p + c, n);
 #pragma unroll
         for (int j = 0; j < V; ++j) out[j] = r[j];
     } else {
-        const auto r = load_words<X, V>((const X *)p + c, n);
+        const auto r = load_words<X, V, ENDS>((const X *)p + c, n);
 #pragma unroll
         for (int j = 0; j < V; ++j) out[j] = r[j];
     }
 }
 
-template <class X, class Y, int G, int K>
+template <class X, class Y, int G, int K, bool ENDS, bool STREAM>
 __global__ __launch_bounds__(kGroup<G>) void layer_norm_forward_kernel(
     const X *__restrict__ x, const void *__restrict__ weight, const void *__restrict__ bias, int params_f32, int cols,
     int64_t rows, int64_t x_stride, float eps, Y *__restrict__ y, float *__restrict__ mean, float *__restrict__ rstd)
@@ -63,35 +94,39 @@ __global__ __launch_bounds__(kGroup<G>) void layer_norm_forward_kernel(
     __shared__ float part[2][G > 64 ? G / 64 : 1];
     const int lane = threadIdx.x % G;
     const int64_t step = (int64_t)gridDim.x * R;
-    int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / G;
+    int64_t row = (int64_t)blockIdx.x * R + row_of_group<G>();
     const float inv = 1.f / (float)cols;
+    int cut[K];
     Words<X, V> next[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int c = (k * G + lane) * V;
-        if (row < rows) next[k] = load_words<X, V>(x + row * x_stride + c, cols - c);
+        cut[k] = cut_by<X, G, ENDS>(cols - c);
+        if (row < rows) next[k] = load_row<X, V, G, ENDS>(x + row * x_stride + c, cols - c, cut[k]);
     }
     float w[K][V], b[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int c = (k * G + lane) * V;
-        load_params<X, V>(weight, params_f32, 1.f, c, cols - c, w[k]);
-        load_params<X, V>(bias, params_f32, 0.f, c, cols - c, b[k]);
+        load_params<X, V, ENDS>(weight, params_f32, 1.f, c, cols - c, w[k]);
+        load_params<X, V, ENDS>(bias, params_f32, 0.f, c, cols - c, b[k]);
     }
     for (; row < rows; row += step) {
         float v[K][V], s = 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            drop_end<G, ENDS>(next[k], cut[k]);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 v[k][j] = next[k][j];
                 s += v[k][j];                       // zero behind the row's end
             }
+        }
         if (row + step < rows) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 const int c = (k * G + lane) * V;
-                next[k] = load_words<X, V>(x + (row + step) * x_stride + c, cols - c);
+                next[k] = load_row<X, V, G, ENDS>(x + (row + step) * x_stride + c, cols - c, cut[k]);
             }
         }
         const float mu = row_sum<G>(s, part[0]) * inv;
@@ -101,7 +136,7 @@ __global__ __launch_bounds__(kGroup<G>) void layer_norm_forward_kernel(
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 v[k][j] -= mu;
-                q += (k * G + lane) * V + j < cols ? v[k][j] * v[k][j] : 0.f;
+                q += (k * G + lane) * V + (ENDS ? j : 0) < cols ? v[k][j] * v[k][j] : 0.f;
             }
         const float r = 1.f / sqrtf(row_sum<G>(q, part[1]) * inv + eps);
 #pragma unroll
@@ -109,7 +144,7 @@ __global__ __launch_bounds__(kGroup<G>) void layer_norm_forward_kernel(
             const int c = (k * G + lane) * V;
 #pragma unroll
             for (int j = 0; j < V; ++j) v[k][j] = v[k][j] * r * w[k][j] + b[k][j];
-            store_pack<Y, V>(y + row * cols + c, v[k], cols - c);
+            store_pack<Y, V, ENDS, STREAM>(y + row * cols + c, v[k], cols - c);
         }
         if (lane == 0) {
             if (mean) mean[row] = mu;
@@ -162,25 +197,37 @@ __global__ __launch_bounds__(kLong) void layer_norm_forward_long_kernel(
     }
 }
 
+// The compiler takes the values for new ones.
+template <class T, int N>
+__device__ inline void forget(Words<T, N> &w)
+{
+#pragma unroll
+    for (int i = 0; i < w.kCount; ++i) asm("" : "+v"(w.w[i]));
+}
+
 // ---- backward, rows in registers --------------------------------------------------------------------
 // One pass over x and dy: dx, and the weights' gradients of the workgroup's rows, which stay in registers until its last
 // row, are added up over the rows that the workgroup has at a time and go to `part` [workgroup][2][cols].  x and dy
 // are held as they were loaded and converted where they are used: with the weight and the two gradients in registers
 // there is no room for the values in fp32 as well, and arithmetic is not what this waits for.
-constexpr int kBack = 1024;
+template <int G>
+constexpr int kBack = G > 512 ? G : 512;
 
-template <class X, class Y, int G, int K>
-__global__ __launch_bounds__(kBack) void layer_norm_backward_kernel(
+template <class X, class Y, int G, int K, bool ENDS, bool STREAM>
+__global__ __launch_bounds__(kBack<G>, 4) void layer_norm_backward_kernel(
     const X *__restrict__ x, const Y *__restrict__ dy, const void *__restrict__ weight, int params_f32, int cols, int64_t rows,
     const float *__restrict__ mean, const float *__restrict__ rstd, int64_t x_stride, int64_t dy_stride, X *__restrict__ dx,
     float *__restrict__ part)
 {
-    constexpr int V = kPack<X>, R = kBack / G, E = K * V;
-    __shared__ float both[2][2][kBack / 64];
+    constexpr int V = kPack<X>, R = kBack<G> / G, E = K * V;
+    __shared__ float both[2][2][kBack<G> / 64];
     const int lane = threadIdx.x % G, wave = threadIdx.x / 64;
     const int64_t step = (int64_t)gridDim.x * R;
-    int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / G;
+    int64_t row = (int64_t)blockIdx.x * R + row_of_group<G>();
     const float inv = 1.f / (float)cols;
+    int cut[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) cut[k] = cut_by<X, G, ENDS>(cols - (k * G + lane) * V);
     Words<X, V> nx[K];
     Words<Y, V> nd[K];
     float nmu, nr;
@@ -190,8 +237,8 @@ __global__ __launch_bounds__(kBack) void layer_norm_backward_kernel(
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = (k * G + lane) * V, n = there ? cols - c : 0;
-            nx[k] = load_words<X, V>(x + at * x_stride + c, n);
-            nd[k] = load_words<Y, V>(dy + at * dy_stride + c, n);
+            nx[k] = load_row<X, V, G, ENDS>(x + at * x_stride + c, n, cut[k]);
+            nd[k] = load_row<Y, V, G, ENDS>(dy + at * dy_stride + c, n, cut[k]);
         }
         nmu = there ? mean[at] : 0.f;
         nr = there ? rstd[at] : 0.f;
@@ -201,7 +248,7 @@ __global__ __launch_bounds__(kBack) void layer_norm_backward_kernel(
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int c = (k * G + lane) * V;
-        load_params<X, V>(weight, params_f32, 1.f, c, cols - c, w + k * V);
+        load_params<X, V, ENDS>(weight, params_f32, 1.f, c, cols - c, w + k * V);
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
@@ -213,6 +260,8 @@ __global__ __launch_bounds__(kBack) void layer_norm_backward_kernel(
         for (int k = 0; k < K; ++k) {
             cx[k] = nx[k];
             cd[k] = nd[k];
+            drop_end<G, ENDS>(cx[k], cut[k]);
+            drop_end<G, ENDS>(cd[k], cut[k]);
         }
         const float mu = nmu, r = nr;
         if (base + step < rows) fetch(row + step);
@@ -247,6 +296,12 @@ __global__ __launch_bounds__(kBack) void layer_norm_backward_kernel(
         }
         su *= inv;
         sh *= inv;
+        // what follows is worked out from x and dy again: kept from above, it would take 16 registers more
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            forget(cx[k]);
+            forget(cd[k]);
+        }
         if (row >= rows) continue;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -257,7 +312,7 @@ __global__ __launch_bounds__(kBack) void layer_norm_backward_kernel(
                 const float h = (cx[k][j] - mu) * r, u = cd[k][j] * w[k * V + j];
                 o[j] = (u - su - h * sh) * r;
             }
-            store_pack<X, V>(dx + row * cols + c, o, cols - c);
+            store_pack<X, V, ENDS, STREAM>(dx + row * cols + c, o, cols - c);
         }
     }
     if (!part) return;
@@ -270,7 +325,7 @@ __global__ __launch_bounds__(kBack) void layer_norm_backward_kernel(
             db[e] += __shfl_xor(db[e], d);
         }
     }
-    constexpr int kTeam = G < 64 ? 64 : G, kHalf = kBack / kTeam / 2;
+    constexpr int kTeam = G < 64 ? 64 : G, kHalf = kBack<G> / kTeam / 2;
     const int team = threadIdx.x / kTeam;
     const bool first = threadIdx.x % kTeam < G;
     if constexpr (kHalf > 0) {
@@ -295,8 +350,8 @@ __global__ __launch_bounds__(kBack) void layer_norm_backward_kernel(
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int c = (k * G + lane) * V;
-        store_pack<float, V>(out + c, dw + k * V, cols - c);
-        store_pack<float, V>(out + cols + c, db + k * V, cols - c);
+        store_pack<float, V, ENDS>(out + c, dw + k * V, cols - c);
+        store_pack<float, V, ENDS>(out + cols + c, db + k * V, cols - c);
     }
 }
 
@@ -429,6 +484,22 @@ int with_back_shape(int64_t cols, F f)
     return f(Shape<0, 0>());
 }
 
+// What a kernel is compiled for: whether a row's end cuts a pack (or only leaves packs out), and whether its output goes
+// past the caches, f(ENDS, STREAM).  The output of a layer is what the next one reads; but where the call reads and
+// writes more than the 256 MB of the last cache, the start of it is gone when that one comes.
+template <bool V>
+struct Bool {
+    static constexpr bool value = V;
+};
+constexpr int64_t kLastCache = (int64_t)256 << 20;
+
+template <class F>
+int with_ends(bool ends, bool stream, F f)
+{
+    if (ends) return stream ? f(Bool<true>(), Bool<true>()) : f(Bool<true>(), Bool<false>());
+    return stream ? f(Bool<false>(), Bool<true>()) : f(Bool<false>(), Bool<false>());
+}
+
 // A workgroup for each set of rows, but no more than the device holds at once: more rows are taken in turn, with the
 // weights in registers and the next row's load on its way.
 uint32_t persistent_groups(int64_t rows, int rows_per_group, int threads)
@@ -463,7 +534,7 @@ int partial_sums(const sv3d_layer_norm_params *p)
         if constexpr (G == 0) {
             return (int)(p->rows < kSlices ? p->rows : kSlices);
         } else {
-            constexpr int R = kBack / G;
+            constexpr int R = kBack<G> / G;
             const int64_t want = (p->rows + R - 1) / R;
             return (int)(want < kBackGroups ? want : kBackGroups);
         }
@@ -494,10 +565,13 @@ extern "C" int sv3d_layer_norm_forward(const sv3d_layer_norm_params *p, const vo
                                    dim3(kLong), 0, (hipStream_t)stream, (const X *)x, weight, bias, f32, cols, p->rows,
                                    p->x_stride, p->eps, (Y *)y, mean, rstd);
             else
-                hipLaunchKernelGGL((layer_norm_forward_kernel<X, Y, G, K>),
-                                   dim3(persistent_groups(p->rows, kGroup<G> / G, kGroup<G>)), dim3(kGroup<G>), 0,
-                                   (hipStream_t)stream, (const X *)x, weight, bias, f32, cols, p->rows, p->x_stride, p->eps,
-                                   (Y *)y, mean, rstd);
+                with_ends(cols % kPack<X> != 0, p->rows * cols * (int64_t)(sizeof(X) + sizeof(Y)) >= kLastCache, [&](auto ends, auto past) {
+                    hipLaunchKernelGGL((layer_norm_forward_kernel<X, Y, G, K, decltype(ends)::value, decltype(past)::value>),
+                                       dim3(persistent_groups(p->rows, kGroup<G> / G, kGroup<G>)), dim3(kGroup<G>), 0,
+                                       (hipStream_t)stream, (const X *)x, weight, bias, f32, cols, p->rows, p->x_stride, p->eps,
+                                       (Y *)y, mean, rstd);
+                    return 0;
+                });
             return launch_status();
         });
     });
@@ -536,9 +610,13 @@ extern "C" int sv3d_layer_norm_backward(const sv3d_layer_norm_params *p, const v
             return with_back_shape<X>(p->cols, [&](auto shape) {
                 constexpr int G = decltype(shape)::G, K = decltype(shape)::K;
                 if constexpr (G > 0) {
-                    hipLaunchKernelGGL((layer_norm_backward_kernel<X, Y, G, K>), dim3(count), dim3(kBack), 0, s,
-                                       (const X *)x, (const Y *)dy, weight, f32, cols, p->rows, mean, rstd, p->x_stride,
-                                       p->dy_stride, (X *)dx, part);
+                    const int64_t bytes = p->rows * cols * (int64_t)(2 * sizeof(X) + sizeof(Y));
+                    with_ends(cols % kPack<X> != 0, bytes >= kLastCache, [&](auto ends, auto past) {
+                        hipLaunchKernelGGL((layer_norm_backward_kernel<X, Y, G, K, decltype(ends)::value, decltype(past)::value>),
+                                           dim3(count), dim3(kBack<G>), 0, s, (const X *)x, (const Y *)dy, weight, f32, cols,
+                                           p->rows, mean, rstd, p->x_stride, p->dy_stride, (X *)dx, part);
+                        return 0;
+                    });
                 } else {
                     if (dx)
                         hipLaunchKernelGGL((layer_norm_dx_long_kernel<X, Y>), dim3(persistent_groups(p->rows, 1, kLong)),
