@@ -1,7 +1,8 @@
 // PyTorch operators of the training step over the C ABI (csrc/norm.hip, csrc/adamw.hip):
 //
-//   layer_norm / layer_norm_backward   layer norm with its own output type; the transformer camera head of the
-//                                      reference's network (nnutils/mesh_net.py:468-536) ends its blocks in one
+//   layer_norm                         layer norm, its result in x's type or float32; the transformer camera head of
+//                                      the reference's network (nnutils/mesh_net.py:468-536) ends its blocks in one
+//   layer_norm_stats / _backward       the same with the rows' statistics, and what they are kept for
 //   grad_square_sums                   squares of a list of gradients, summed (the norm that clipping needs)
 //   adamw_step                         unscale, clip and AdamW over a list of tensors (nnutils/train_utils.py:201-214),
 //                                      32-bit or 8-bit moments
@@ -96,31 +97,59 @@ int32_t code_of(at::ScalarType t) { return t == at::kFloat ? SV3D_F32 : t == at:
 
 using NormOut = std::tuple<Tensor, Tensor, Tensor>;
 
-NormOut layer_norm_gpu(const Tensor &x, IntList shape, const optional<Tensor> &weight, const optional<Tensor> &bias,
-                       double eps, bool f32_out, bool stats)
+// mean and rstd may be undefined: nobody will call the backward
+void run_layer_norm(const Tensor &x, int64_t cols, const optional<Tensor> &weight, const optional<Tensor> &bias, double eps,
+                    Tensor &y, Tensor *mean, Tensor *rstd)
 {
-    const int64_t cols = check_norm(x, shape, weight, bias);
     TORCH_CHECK_VALUE(eps >= 0.0, "eps must not be negative, got ", eps);
     Launch L(x);
     const Rows r = rows_of(x, cols);
     const auto pt = param_type(x, weight, bias);
     const Tensor w = as_param(weight, pt), b = as_param(bias, pt);
-    Tensor y = at::empty(x.sizes(), x.options().dtype(f32_out ? at::kFloat : x.scalar_type()));
-    Tensor mean = at::empty({stats ? r.count : 0}, x.options().dtype(at::kFloat)), rstd = at::empty_like(mean);
     const sv3d_layer_norm_params p = {r.count, cols, r.stride, cols, code_of(x.scalar_type()), code_of(y.scalar_type()),
                                       code_of(pt), (float)eps};
-    check_status(sv3d_layer_norm_forward(&p, ptr(r.t), ptr(w), ptr(b), ptr(y), (float *)ptr(mean), (float *)ptr(rstd), L.stream),
+    check_status(sv3d_layer_norm_forward(&p, ptr(r.t), ptr(w), ptr(b), ptr(y), mean ? (float *)ptr(*mean) : nullptr,
+                                         rstd ? (float *)ptr(*rstd) : nullptr, L.stream),
                  "sv3d_layer_norm_forward");
+}
+
+Tensor norm_output(const Tensor &x, bool f32_out)
+{
+    return at::empty(x.sizes(), x.options().dtype(f32_out ? at::kFloat : x.scalar_type()));
+}
+
+Tensor layer_norm_gpu(const Tensor &x, IntList shape, const optional<Tensor> &weight, const optional<Tensor> &bias, double eps,
+                      bool f32_out)
+{
+    const int64_t cols = check_norm(x, shape, weight, bias);
+    Tensor y = norm_output(x, f32_out);
+    run_layer_norm(x, cols, weight, bias, eps, y, nullptr, nullptr);
+    return y;
+}
+
+Tensor layer_norm_meta(const Tensor &x, IntList shape, const optional<Tensor> &weight, const optional<Tensor> &bias, double,
+                       bool f32_out)
+{
+    check_norm(x, shape, weight, bias);
+    return norm_output(x, f32_out);
+}
+
+NormOut layer_norm_stats_gpu(const Tensor &x, IntList shape, const optional<Tensor> &weight, const optional<Tensor> &bias,
+                             double eps, bool f32_out)
+{
+    const int64_t cols = check_norm(x, shape, weight, bias);
+    Tensor y = norm_output(x, f32_out);
+    Tensor mean = at::empty({x.numel() / cols}, x.options().dtype(at::kFloat)), rstd = at::empty_like(mean);
+    run_layer_norm(x, cols, weight, bias, eps, y, &mean, &rstd);
     return {y, mean, rstd};
 }
 
-NormOut layer_norm_meta(const Tensor &x, IntList shape, const optional<Tensor> &weight, const optional<Tensor> &bias,
-                        double, bool f32_out, bool stats)
+NormOut layer_norm_stats_meta(const Tensor &x, IntList shape, const optional<Tensor> &weight, const optional<Tensor> &bias,
+                              double, bool f32_out)
 {
     const int64_t cols = check_norm(x, shape, weight, bias);
-    Tensor y = at::empty(x.sizes(), x.options().dtype(f32_out ? at::kFloat : x.scalar_type()));
-    Tensor mean = at::empty({stats ? x.numel() / cols : 0}, x.options().dtype(at::kFloat));
-    return {y, mean, at::empty_like(mean)};
+    Tensor mean = at::empty({x.numel() / cols}, x.options().dtype(at::kFloat));
+    return {norm_output(x, f32_out), mean, at::empty_like(mean)};
 }
 
 void check_norm_backward(const Tensor &dy, const Tensor &x, int64_t cols, const Tensor &mean, const Tensor &rstd)
@@ -180,28 +209,21 @@ NormOut layer_norm_backward_meta(const Tensor &dy, const Tensor &x, IntList shap
             need_bias ? at::empty(shape, x.options().dtype(given(bias) ? bias->scalar_type() : pt)) : none()};
 }
 
-NormOut call_layer_norm(const Tensor &x, IntList shape, const optional<Tensor> &weight, const optional<Tensor> &bias,
-                        double eps, bool f32_out, bool stats)
-{
-    static auto op = find_op<NormOut(const Tensor &, IntList, const optional<Tensor> &, const optional<Tensor> &, double, bool,
-                                     bool)>("sv3d::layer_norm");
-    return op.call(x, shape, weight, bias, eps, f32_out, stats);
-}
-
 struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
-    static variable_list forward(AutogradContext *ctx, const Tensor &x, IntList shape, const optional<Tensor> &weight,
-                                 const optional<Tensor> &bias, double eps, bool f32_out)
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, IntList shape, const optional<Tensor> &weight,
+                          const optional<Tensor> &bias, double eps, bool f32_out)
     {
         at::AutoDispatchBelowADInplaceOrView guard;
-        auto out = call_layer_norm(x, shape, weight, bias, eps, f32_out, true);
+        static auto op = find_op<NormOut(const Tensor &, IntList, const optional<Tensor> &, const optional<Tensor> &, double,
+                                         bool)>("sv3d::layer_norm_stats");
+        auto out = op.call(x, shape, weight, bias, eps, f32_out);
         ctx->save_for_backward({x, given(weight) ? *weight : Tensor(), given(bias) ? *bias : Tensor(), std::get<1>(out),
                                 std::get<2>(out)});
-        ctx->saved_data["shape"] = shape.vec();
-        ctx->saved_data["need"] = std::vector<int64_t>{x.requires_grad(), given(weight) && weight->requires_grad(),
-                                                       given(bias) && bias->requires_grad()};
-        ctx->mark_non_differentiable({std::get<1>(out), std::get<2>(out)});
+        ctx->saved_data["shape"] = shape;
+        ctx->saved_data["need"] = (int64_t)((x.requires_grad() ? 1 : 0) | (given(weight) && weight->requires_grad() ? 2 : 0) |
+                                            (given(bias) && bias->requires_grad() ? 4 : 0));
         ctx->set_materialize_grads(false);
-        return {std::get<0>(out), std::get<1>(out), std::get<2>(out)};
+        return std::get<0>(out);
     }
 
     static variable_list backward(AutogradContext *ctx, variable_list grads)
@@ -210,33 +232,33 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
         TORCH_CHECK(!at::GradMode::is_enabled(), "sv3d::layer_norm has no second derivative (create_graph=True)");
         const auto s = ctx->get_saved_variables();
         const auto shape = ctx->saved_data["shape"].toIntVector();
-        const auto need = ctx->saved_data["need"].toIntVector();
+        const int64_t need = ctx->saved_data["need"].toInt();
         optional<Tensor> weight, bias;
         if (s[1].defined()) weight = s[1];
         if (s[2].defined()) bias = s[2];
         static auto op = find_op<NormOut(const Tensor &, const Tensor &, IntList, const optional<Tensor> &,
                                          const optional<Tensor> &, const Tensor &, const Tensor &, bool, bool, bool)>(
             "sv3d::layer_norm_backward");
-        auto g = op.call(grads[0], s[0], shape, weight, bias, s[3], s[4], need[0], need[1], need[2]);
+        auto g = op.call(grads[0], s[0], shape, weight, bias, s[3], s[4], (need & 1) != 0, (need & 2) != 0, (need & 4) != 0);
         variable_list out(6);
-        if (need[0]) out[0] = std::get<0>(g);
-        if (need[1]) out[2] = std::get<1>(g);
-        if (need[2]) out[3] = std::get<2>(g);
+        if (need & 1) out[0] = std::get<0>(g);
+        if (need & 2) out[2] = std::get<1>(g);
+        if (need & 4) out[3] = std::get<2>(g);
         return out;
     }
 };
 
-NormOut layer_norm_autograd(const Tensor &x, IntList shape, const optional<Tensor> &weight, const optional<Tensor> &bias,
-                            double eps, bool f32_out, bool stats)
+Tensor layer_norm_autograd(const Tensor &x, IntList shape, const optional<Tensor> &weight, const optional<Tensor> &bias,
+                           double eps, bool f32_out)
 {
     const bool wanted = at::GradMode::is_enabled() && (x.requires_grad() || (given(weight) && weight->requires_grad()) ||
                                                        (given(bias) && bias->requires_grad()));
-    if (!wanted) {
-        at::AutoDispatchBelowADInplaceOrView guard;
-        return call_layer_norm(x, shape, weight, bias, eps, f32_out, stats);
-    }
-    auto out = LayerNormFn::apply(x, shape, weight, bias, eps, f32_out);
-    return {out[0], out[1], out[2]};
+    if (wanted) return LayerNormFn::apply(x, shape, weight, bias, eps, f32_out);
+    // no gradient will be asked for: without the statistics of the rows
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static auto op = find_op<Tensor(const Tensor &, IntList, const optional<Tensor> &, const optional<Tensor> &, double, bool)>(
+        "sv3d::layer_norm");
+    return op.call(x, shape, weight, bias, eps, f32_out);
 }
 
 // ---- optimizer ------------------------------------------------------------------------------------
@@ -426,6 +448,25 @@ Tensor adamw_step_meta(TensorList params, TensorList grads, TensorList exp_avgs,
     return at::empty({}, params[0].options().dtype(at::kFloat));
 }
 
+// Without kernels of their own these operators would pass autograd's generic check, which takes the lists apart once more (30 us
+// for 72 tensors).
+Tensor adamw_step_autograd(TensorList params, TensorList grads, TensorList exp_avgs, TensorList exp_avg_sqs, TensorList scales,
+                           TensorList steps, const optional<Tensor> &lr_tensor, const optional<Tensor> &grad_scale,
+                           const optional<Tensor> &found_inf, const optional<Tensor> &square_sums, double lr, double beta1,
+                           double beta2, double eps, double weight_decay, double max_norm, bool maximize, int64_t seed)
+{
+    if (at::GradMode::is_enabled())
+        for (const auto *tensors : {&params, &exp_avgs, &exp_avg_sqs})
+            for (const Tensor &t : *tensors)
+                TORCH_CHECK(!t.requires_grad(), "sv3d::adamw_step changes tensors that require a gradient: call it under torch.no_grad()");
+    at::AutoDispatchBelowADInplaceOrView guard;
+    using O = const optional<Tensor> &;
+    static auto op = find_op<Tensor(TensorList, TensorList, TensorList, TensorList, TensorList, TensorList, O, O, O, O, double,
+                                    double, double, double, double, double, bool, int64_t)>("sv3d::adamw_step");
+    return op.call(params, grads, exp_avgs, exp_avg_sqs, scales, steps, lr_tensor, grad_scale, found_inf, square_sums, lr, beta1,
+                   beta2, eps, weight_decay, max_norm, maximize, seed);
+}
+
 int64_t check_moments(const Tensor &exp_avg, const Tensor &exp_avg_sq, const Tensor &scales)
 {
     TORCH_CHECK_VALUE(exp_avg.scalar_type() == at::kByte && exp_avg_sq.scalar_type() == at::kByte && same_layout(exp_avg, exp_avg_sq) &&
@@ -461,7 +502,8 @@ std::tuple<Tensor, Tensor> moment_values_meta(const Tensor &exp_avg, const Tenso
 
 TORCH_LIBRARY_FRAGMENT(sv3d, m)
 {
-    m.def("layer_norm(Tensor x, int[] normalized_shape, Tensor? weight, Tensor? bias, float eps, bool f32_out, bool stats) "
+    m.def("layer_norm(Tensor x, int[] normalized_shape, Tensor? weight, Tensor? bias, float eps, bool f32_out) -> Tensor");
+    m.def("layer_norm_stats(Tensor x, int[] normalized_shape, Tensor? weight, Tensor? bias, float eps, bool f32_out) "
           "-> (Tensor, Tensor, Tensor)");
     m.def("layer_norm_backward(Tensor grad_y, Tensor x, int[] normalized_shape, Tensor? weight, Tensor? bias, Tensor mean, "
           "Tensor rstd, bool need_x, bool need_weight, bool need_bias) -> (Tensor, Tensor, Tensor)");
@@ -476,6 +518,7 @@ TORCH_LIBRARY_FRAGMENT(sv3d, m)
 TORCH_LIBRARY_IMPL(sv3d, CUDA, m)
 {
     m.impl("layer_norm", layer_norm_gpu);
+    m.impl("layer_norm_stats", layer_norm_stats_gpu);
     m.impl("layer_norm_backward", layer_norm_backward_gpu);
     m.impl("grad_square_sums", grad_square_sums_gpu);
     m.impl("adamw_step", adamw_step_gpu);
@@ -485,6 +528,7 @@ TORCH_LIBRARY_IMPL(sv3d, CUDA, m)
 TORCH_LIBRARY_IMPL(sv3d, Meta, m)
 {
     m.impl("layer_norm", layer_norm_meta);
+    m.impl("layer_norm_stats", layer_norm_stats_meta);
     m.impl("layer_norm_backward", layer_norm_backward_meta);
     m.impl("grad_square_sums", grad_square_sums_meta);
     m.impl("adamw_step", adamw_step_meta);
@@ -494,4 +538,10 @@ TORCH_LIBRARY_IMPL(sv3d, Meta, m)
 TORCH_LIBRARY_IMPL(sv3d, Autograd, m)
 {
     m.impl("layer_norm", layer_norm_autograd);
+    m.impl("adamw_step", adamw_step_autograd);
+    // no gradients: what comes back requires none
+    m.impl("layer_norm_stats", torch::CppFunction::makeFallthrough());
+    m.impl("layer_norm_backward", torch::CppFunction::makeFallthrough());
+    m.impl("grad_square_sums", torch::CppFunction::makeFallthrough());
+    m.impl("moment_values", torch::CppFunction::makeFallthrough());
 }

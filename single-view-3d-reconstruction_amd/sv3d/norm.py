@@ -1,11 +1,11 @@
-"""Layer norm on the device: entry point of the operators `sv3d::layer_norm` / `sv3d::layer_norm_backward`
+"""Layer norm on the device: entry point of the operators `sv3d::layer_norm`, `sv3d::layer_norm_stats` and `sv3d::layer_norm_backward`
 (csrc/torch_train_ops.cpp over the functions of the same names in include/sv3d_hip.h), and the module over it.
 The transformer camera head of the reference's network (nnutils/mesh_net.py:468-536) is made of blocks that each
 end in one.  GPU tensors only.
 """
 import torch
 
-from .ops import _ops
+from .ops import call
 
 
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
@@ -14,10 +14,8 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     scales and shifts by `weight` and `bias` (of x's type or float32).  Statistics, arithmetic and the sums of the
     weights' gradients are float32; the result has x's type, under autocast float32 (as torch's).  Differentiable
     once in x, weight and bias."""
-    shape = [normalized_shape] if isinstance(normalized_shape, int) else list(normalized_shape)
-    need = torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                        or (bias is not None and bias.requires_grad))
-    return _ops.layer_norm(x, shape, weight, bias, eps, torch.is_autocast_enabled("cuda"), need)[0]
+    shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
+    return call("layer_norm", x, shape, weight, bias, eps, torch.is_autocast_enabled("cuda"))
 
 
 class LayerNorm(torch.nn.LayerNorm):

@@ -39,6 +39,29 @@ def _load_torch_ops():
 _ops = _load_torch_ops()
 
 
+def _load_calls():
+    try:
+        from . import _call
+    except ImportError as e:
+        raise L.Sv3dError(
+            "sv3d/_call.so cannot be loaded (%s): build it with `python -c 'import __graft_entry__ as g; g.build()'` or "
+            "`make -C single-view-3d-reconstruction_amd/csrc`; there is no fallback path" % e) from e
+    return _call
+
+
+_call = _load_calls()
+
+
+def call(name, *args):
+    """The operator `name` of those that `_call` has, with all its arguments in their order: directly, or through torch.ops
+    where that is needed (arguments that are not plain tensors, tracing by torch.compile)."""
+    if not torch.compiler.is_compiling():
+        out = getattr(_call, name)(*args)
+        if out is not NotImplemented:
+            return out
+    return getattr(_ops, name)(*args)
+
+
 # ---- argument packing --------------------------------------------------------------------------
 _MODES = {"surface": L.SV3D_TEX_SURFACE, "vertex": L.SV3D_TEX_VERTEX, "vertex8": L.SV3D_TEX_VERTEX8}
 

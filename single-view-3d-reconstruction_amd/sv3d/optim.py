@@ -5,14 +5,14 @@ the optimizer over them.  It does in two passes over the gradients what the refe
 """
 import torch
 
-from .ops import _ops
+from .ops import _ops, call
 
 STATE_BLOCK = 128           # elements that share the scales of their 8-bit moments
 
 
 def grad_square_sums(grads):
     """Sums of squares of the listed gradients in float64, as several numbers (`.sum().sqrt()` is their norm)."""
-    return _ops.grad_square_sums(grads)
+    return call("grad_square_sums", grads)
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, scales=None, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
@@ -37,9 +37,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, scales=None, lr=1
         raise ValueError("max_norm must not be negative or NaN, got %r" % (max_norm,))
     with torch.no_grad():
         if clip and square_sums is None:
-            square_sums = _ops.grad_square_sums(grads)
+            square_sums = call("grad_square_sums", grads)
         tensor_lr = lr if torch.is_tensor(lr) else None
-        norm = _ops.adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales if scales is not None else [], steps, tensor_lr,
+        norm = call("adamw_step", params, grads, exp_avgs, exp_avg_sqs, scales if scales is not None else [], steps, tensor_lr,
                                grad_scale, found_inf, square_sums if clip else None, 0.0 if tensor_lr is not None else lr,
                                betas[0], betas[1], eps, weight_decay, max_norm if clip else 0.0, maximize, seed)
     return norm if clip else None

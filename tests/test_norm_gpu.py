@@ -305,8 +305,8 @@ def test_operator_registration():
     x, w, b, dy = (t.cuda() for t in make(4, 32))
     for a in (x, w, b):
         a.requires_grad_()
-    torch.library.opcheck(torch.ops.sv3d.layer_norm.default, (x, [32], w, b, 1e-5, False, True), test_utils=tests)
-    _, mean, rstd = torch.ops.sv3d.layer_norm(x.detach(), [32], None, None, 1e-5, False, True)
+    torch.library.opcheck(torch.ops.sv3d.layer_norm.default, (x, [32], w, b, 1e-5, False), test_utils=tests)
+    _, mean, rstd = torch.ops.sv3d.layer_norm_stats(x.detach(), [32], None, None, 1e-5, False)
     torch.library.opcheck(torch.ops.sv3d.layer_norm_backward.default,
                           (dy, x.detach(), [32], None, None, mean, rstd, True, True, True), test_utils=("test_schema", "test_faketensor"))
 
@@ -322,7 +322,7 @@ def test_more_elements_than_32_bits_count():
     f = to.layer_norm(wide(x[-3:]), None, None, 1e-5)
     assert_near(y[-3:], f["y"], f["e_y"])
     del y
-    _, mean, rstd = torch.ops.sv3d.layer_norm(x, [cols], None, None, 1e-5, False, True)
+    _, mean, rstd = torch.ops.sv3d.layer_norm_stats(x, [cols], None, None, 1e-5, False)
     dx, _, _ = torch.ops.sv3d.layer_norm_backward(x, x, [cols], None, None, mean, rstd, True, False, False)
     assert torch.equal(dx[:3], dx[-3:])
     back = to.layer_norm_backward(f, wide(x[-3:]), None)

@@ -91,10 +91,10 @@ def test_layer_norm_refuses(x, shape, weight, bias, eps):
 
 
 def test_layer_norm_shapes_and_types_without_a_gpu():
-    y, mean, rstd = torch.ops.sv3d.layer_norm(meta(2, 3, 8, dtype=torch.bfloat16), [3, 8], None, None, 1e-5, False, True)
+    y, mean, rstd = torch.ops.sv3d.layer_norm_stats(meta(2, 3, 8, dtype=torch.bfloat16), [3, 8], None, None, 1e-5, False)
     assert y.shape == (2, 3, 8) and y.dtype == torch.bfloat16 and mean.shape == rstd.shape == (2,)
-    y, mean, _ = torch.ops.sv3d.layer_norm(meta(2, 8, dtype=torch.float16), [8], meta(8), None, 1e-5, True, False)
-    assert y.dtype == torch.float32 and mean.numel() == 0
+    y = torch.ops.sv3d.layer_norm(meta(2, 8, dtype=torch.float16), [8], meta(8), None, 1e-5, True)
+    assert y.dtype == torch.float32 and y.shape == (2, 8)
     with pytest.raises(NotImplementedError):
         norm.layer_norm(torch.zeros(2, 8), 8)
     with pytest.raises(ValueError):             # statistics of another call
@@ -291,3 +291,33 @@ def test_trainer_on_the_host_refuses_what_needs_a_gpu(tmp_path, argv, error):
     o = train_utils.add_training_flags().parse_args(["--checkpoint_dir", str(tmp_path), *argv])
     with pytest.raises(error):
         T(o, env=train_utils.DistEnv()).init_training()
+
+
+def test_operators_see_the_same_through_torch_ops_and_directly():
+    """What `sv3d._call` hands back to torch.ops (a mode that wants to see every function) and what it takes itself."""
+    from torch.overrides import TorchFunctionMode
+    from sv3d import ops
+
+    class Watch(TorchFunctionMode):
+        seen = 0
+
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            Watch.seen += 1
+            return func(*args, **(kwargs or {}))
+
+    x = meta(2, 8)
+    with Watch():
+        y = norm.layer_norm(x, 8)
+    assert Watch.seen > 0 and y.shape == x.shape
+    args = (x, (8,), None, None, 1e-5, False)
+    assert ops._call.layer_norm(*args).shape == (2, 8)
+    assert ops._call.layer_norm(*args[:-1]) is NotImplemented
+    assert ops._call.layer_norm([x], *args[1:]) is NotImplemented
+    assert ops._call.layer_norm(x, 8, *args[2:]) is NotImplemented
+    assert ops._call.grad_square_sums((x, None)) is NotImplemented
+    assert ops._call.grad_square_sums((x, x)).dtype == torch.float64
+    p = torch.nn.Parameter(meta(5))
+    with pytest.raises(RuntimeError, match="no_grad"):
+        torch.ops.sv3d.adamw_step([p], [meta(5)], [meta(5)], [meta(5)], [], [meta()], None, None, None, None, 1e-3, 0.9, 0.9,
+                                  1e-8, 0.0, 0.0, False, 0)
+    assert optim.adamw_step([p], [meta(5)], [meta(5)], [meta(5)], [meta()]) is None
