@@ -300,6 +300,28 @@ def test_no_second_derivative_and_no_change_after_the_forward():
         torch.autograd.grad(y, x, dy)
 
 
+def test_the_graph_can_be_kept_used_in_part_and_only_once():
+    x, w, b, dy = (t.cuda() for t in make(6, 40))
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    y = sv3d.layer_norm(leaves[0], 40, leaves[1], leaves[2])
+    assert y.requires_grad and "LayerNormBackward" in y.grad_fn.name()
+    first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    only_w, = torch.autograd.grad(y, leaves[1:2], dy, retain_graph=True)
+    again = torch.autograd.grad(y, leaves, dy)
+    assert torch.equal(only_w, first[1]) and all(torch.equal(a, e) for a, e in zip(again, first))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, leaves, dy)
+    # through checkpointing, whose hooks take the saved tensors away and recompute them
+    from torch.utils.checkpoint import checkpoint
+    y = checkpoint(lambda a: sv3d.layer_norm(a * 1, 40, leaves[1], leaves[2]), leaves[0], use_reentrant=False)
+    assert all(torch.equal(a, e) for a, e in zip(torch.autograd.grad(y, leaves, dy), first))
+    for t in leaves:
+        t.grad = None
+    (sv3d.layer_norm(leaves[0], 40, leaves[1], leaves[2]) * dy).sum().backward()
+    (sv3d.layer_norm(leaves[0], 40, leaves[1], leaves[2]) * dy).sum().backward()
+    assert all(torch.equal(t.grad, 2 * e) for t, e in zip(leaves, first))       # accumulated: twice the same bits
+
+
 def test_operator_registration():
     tests = ("test_schema", "test_autograd_registration", "test_faketensor")
     x, w, b, dy = (t.cuda() for t in make(4, 32))
