@@ -389,14 +389,16 @@ int sv3d_grad_square_sums_count(const sv3d_adamw_tensor *tensors, int32_t num_te
 int sv3d_grad_square_sums(const sv3d_adamw_tensor *tensors, int32_t num_tensors, double *sums, int32_t count,
                           void *stream);
 
-/* With S = *grad_scale (1 if NULL), G = sqrt(sum of square_sums) / S and
- *   g  = grad / S * min(1, max_norm / (G + 1e-6))       (no factor if square_sums is NULL)
+/* With S = *grad_scale (1 if NULL), G = the norm of all gradients of the call divided by S (or
+ * sqrt(sum of square_sums) / S where square_sums is not NULL) and
+ *   g  = grad / S * min(1, max_norm / (G + 1e-6))       (no factor if max_norm is 0)
  *   t  = step + 1;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   param = param (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
- * in fp32 (an eps below 2^-63 counts as 2^-63); the weight is rounded to its type to nearest, 8-bit moments are rounded up or down with the
- * probability of what is cut off, decided by a hash of (element, t, seed), and a positive exp_avg_sq
- * never becomes zero.  `maximize` negates g.  If *found_inf is not 0 nothing is changed.  lr is read from
- * `lr_device` where that is not NULL.  *total_norm (may be NULL) receives G.
+ * in fp32 (an eps below 2^-63 counts as 2^-63); the weight is rounded to its type to nearest, 8-bit
+ * moments are rounded up or down with the probability of what is cut off, decided by a hash of
+ * (element, t, seed), and a positive exp_avg_sq never becomes zero.  `maximize` negates g.  If *found_inf is
+ * not 0 nothing is changed.  lr is read from `lr_device` where that is not NULL.  With max_norm > 0
+ * *total_norm (may be NULL) receives G.
  * `workspace`: sv3d_adamw_workspace() bytes, 16-byte aligned; its content does not matter. */
 typedef struct sv3d_adamw_params {
     double lr, beta1, beta2, eps, weight_decay, max_norm;
@@ -410,7 +412,7 @@ typedef struct sv3d_adamw_params {
     uint32_t seed;
 } sv3d_adamw_params;
 
-int sv3d_adamw_workspace(int32_t num_tensors, size_t *bytes);
+int sv3d_adamw_workspace(const sv3d_adamw_params *p, const sv3d_adamw_tensor *tensors, int32_t num_tensors, size_t *bytes);
 int sv3d_adamw_step(const sv3d_adamw_params *p, const sv3d_adamw_tensor *tensors, int32_t num_tensors,
                     void *workspace, size_t workspace_bytes, void *stream);
 

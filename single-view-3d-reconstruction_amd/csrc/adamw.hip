@@ -5,6 +5,7 @@
 // be kept up to date), at most kTable of them per launch, cut into chunks; a workgroup looks up its chunk's tensor.
 #include "element.h"
 
+#include <cmath>
 #include <type_traits>
 
 // fused products and sums are written out: the same bits wherever a function is inlined
@@ -24,6 +25,17 @@ constexpr int kChunk8 = 2048;       // 8-bit moments
 constexpr int kBlock = SV3D_STATE_BLOCK;
 constexpr int kSumChunk = 4096;
 constexpr int kSumGroups = 1024;
+
+// the sum over a workgroup's threads, known to thread 0; `part`: one number per wave
+__device__ inline double group_sum(double v, double *part, int waves)
+{
+    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = v;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        for (int w = 1; w < waves; ++w) v += part[w];
+    return v;
+}
 
 // ---- the norm: sums of squares --------------------------------------------------------------------
 // Squares and sums in double: a square of an fp32 number neither overflows nor is rounded there, and the order of
@@ -65,14 +77,8 @@ __global__ __launch_bounds__(kThreads) void grad_square_sums_kernel(SumTable t, 
 #pragma unroll
             for (int j = 0; j < V; ++j) acc[j & 3] += (double)w[u][j] * (double)w[u][j];
     }
-    double sum = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kThreads / 64; ++w) sum += part[w];
-        sums[blockIdx.x] = sum;
-    }
+    const double sum = group_sum((acc[0] + acc[1]) + (acc[2] + acc[3]), part, kThreads / 64);
+    if (threadIdx.x == 0) sums[blockIdx.x] = sum;
 }
 
 // ---- what each tensor's update multiplies by -------------------------------------------------------
@@ -86,51 +92,66 @@ struct Factors {
     int32_t pad[2];
 };
 
+// What the kernels need of the call's parameters.
+struct Scalars {
+    double lr, log_b1, log_b2, weight_decay, max_norm;
+    const float *lr_device, *grad_scale, *found_inf;
+    float *total_norm;
+    uint32_t seed;
+    int32_t maximize;
+};
+
+// What gradients are multiplied by, from the sum of their squares (or none of it); one thread of a call.
+__device__ inline double grad_factor(const Scalars &p, double square_sum)
+{
+    const double inv = p.grad_scale ? 1.0 / (double)*p.grad_scale : 1.0;
+    double c = 1.0;
+    if (p.max_norm > 0.0) {
+        const double norm = sqrt(square_sum) * inv;
+        if (p.total_norm) *p.total_norm = (float)norm;
+        c = p.max_norm / (norm + 1e-6);
+        if (c > 1.0) c = 1.0;                   // a norm that is no number goes through, into every weight
+    }
+    return (p.maximize ? -inv : inv) * c;
+}
+
+// Takes a tensor's step count forward.  In double: beta^t close to 1 is subtracted from 1.
+__device__ inline Factors factors_of(const Scalars &p, float *step, double grad)
+{
+    const int32_t skip = p.found_inf && *p.found_inf != 0.f;
+    const double lr = p.lr_device ? (double)*p.lr_device : p.lr;
+    const float n = *step + 1.f;
+    if (!skip) *step = n;
+    Factors f;
+    f.grad = (float)grad;
+    f.decay = (float)(1.0 - lr * p.weight_decay);
+    f.rate = (float)(lr / -expm1((double)n * p.log_b1));
+    f.root = (float)(1.0 / sqrt(-expm1((double)n * p.log_b2)));
+    f.key = (uint32_t)n * 0x9E3779B1u + p.seed * 0x6A09E667u;
+    f.skip = skip;
+    f.pad[0] = f.pad[1] = 0;
+    return f;
+}
+
 constexpr int kSteps = 384;
 struct StepTable {
     float *step[kSteps];
     int32_t base, count;
 };
+static_assert(sizeof(StepTable) + sizeof(Scalars) + 32 <= 4096, "kernel arguments");
 
-// One workgroup.  Takes the step counts forward, in double: beta^t close to 1 is subtracted from 1.
-__global__ __launch_bounds__(kThreads) void adamw_factors_kernel(StepTable t, sv3d_adamw_params p, Factors *__restrict__ out)
+// One workgroup: the factors of up to kSteps tensors.
+__global__ __launch_bounds__(kThreads) void adamw_factors_kernel(StepTable t, Scalars p, const double *__restrict__ sums,
+                                                                 int num_sums, Factors *__restrict__ out)
 {
     __shared__ double part[kThreads / 64];
-    __shared__ double scale;
-    const double inv = p.grad_scale ? 1.0 / (double)*p.grad_scale : 1.0;
-    if (p.square_sums) {
-        double acc = 0.0;
-        for (int i = threadIdx.x; i < p.num_square_sums; i += kThreads) acc += p.square_sums[i];
-        for (int d = 32; d > 0; d >>= 1) acc += __shfl_xor(acc, d);
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = acc;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < kThreads / 64; ++w) acc += part[w];
-            const double norm = sqrt(acc) * inv;
-            if (p.total_norm) *p.total_norm = (float)norm;
-            const double c = p.max_norm / (norm + 1e-6);
-            scale = inv * (c > 1.0 ? 1.0 : c);      // a norm that is no number goes through, into every weight
-        }
-        __syncthreads();
-    } else {
-        if (threadIdx.x == 0) scale = inv;
-        __syncthreads();
-    }
-    const int32_t skip = p.found_inf && *p.found_inf != 0.f;
-    const double lr = p.lr_device ? (double)*p.lr_device : p.lr;
-    for (int i = threadIdx.x; i < t.count; i += kThreads) {
-        const float n = *t.step[i] + 1.f;
-        if (!skip) *t.step[i] = n;
-        Factors f;
-        f.grad = (float)(p.maximize ? -scale : scale);
-        f.decay = (float)(1.0 - lr * p.weight_decay);
-        f.rate = (float)(lr / (1.0 - pow(p.beta1, (double)n)));
-        f.root = (float)(1.0 / sqrt(1.0 - pow(p.beta2, (double)n)));
-        f.key = (uint32_t)n * 0x9E3779B1u + p.seed * 0x6A09E667u;
-        f.skip = skip;
-        f.pad[0] = f.pad[1] = 0;
-        out[t.base + i] = f;
-    }
+    __shared__ double grad;
+    double acc = 0.0;
+    for (int i = threadIdx.x; i < num_sums; i += kThreads) acc += sums[i];
+    acc = group_sum(acc, part, kThreads / 64);
+    if (threadIdx.x == 0) grad = grad_factor(p, acc);
+    __syncthreads();
+    for (int i = threadIdx.x; i < t.count; i += kThreads) out[t.base + i] = factors_of(p, t.step[i], grad);
 }
 
 // ---- 8-bit moments -----------------------------------------------------------------------------------
@@ -253,12 +274,14 @@ __device__ inline float step_of(float p, float &m, float &v, float g, const Beta
 }
 
 // The tensor of chunk `chunk`: the lanes look at the table's entries at once, two each.
+template <int TABLE>
 __device__ inline int tensor_of(const int32_t *first, int count, int chunk)
 {
-    static_assert(kTable > 64 && kTable <= 128, "two entries per lane");
+    static_assert(TABLE <= 128, "two entries per lane");
     const int lane = threadIdx.x & 63;
-    return __popcll(__ballot(lane < count && chunk >= first[lane + 1])) +
-           __popcll(__ballot(lane + 64 < count && chunk >= first[min(lane + 65, kTable)]));
+    int k = __popcll(__ballot(lane < count && chunk >= first[lane + 1]));
+    if (TABLE > 64) k += __popcll(__ballot(lane + 64 < count && chunk >= first[min(lane + 65, TABLE)]));
+    return k;
 }
 
 // A whole chunk's loads go out together; with the ends checked they would wait for each other, which only a tensor's last
@@ -322,7 +345,7 @@ __device__ inline void update_chunk(const Entry &e, int64_t at, int left, const 
 template <class T, bool STREAM_G>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(Table t, Betas b, const Factors *__restrict__ factors)
 {
-    const int chunk = blockIdx.x, k = __builtin_amdgcn_readfirstlane(tensor_of(t.first, t.count, chunk));
+    const int chunk = blockIdx.x, k = __builtin_amdgcn_readfirstlane(tensor_of<kTable>(t.first, t.count, chunk));
     const Factors f = factors[t.order[k]];
     if (f.skip) return;
     const int64_t from = (int64_t)(chunk - t.first[k]) * kChunk, left = (int64_t)t.numel[k] - from;
@@ -412,7 +435,7 @@ __device__ inline void update_chunk8(const Entry &e, int64_t at, int n, uint32_t
 template <class T, bool STREAM_G>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(Table t, Betas b, const Factors *__restrict__ factors)
 {
-    const int chunk = blockIdx.x, k = __builtin_amdgcn_readfirstlane(tensor_of(t.first, t.count, chunk));
+    const int chunk = blockIdx.x, k = __builtin_amdgcn_readfirstlane(tensor_of<kTable>(t.first, t.count, chunk));
     const Factors f = factors[t.order[k]];
     if (f.skip) return;
     const int64_t from = (int64_t)(chunk - t.first[k]) * kChunk8, left = (int64_t)t.numel[k] - from;
@@ -424,6 +447,62 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(Table t, Betas b, cons
         // the 16 lanes of a block stay or go together: each of them passes on what others found
         if (mine / kBlock * kBlock >= left) return;
         update_chunk8<false, STREAM_G, T>(t.t[k], from + mine, (int)left - mine, element, b, f);
+    }
+}
+
+// ---- small calls: everything in one workgroup, one launch ----------------------------------------------
+// The norm, the factors and the update of at most kSmallChunks chunks: four teams of 256 threads take a chunk each.
+constexpr int kSmallThreads = 1024, kSmallTable = 64;
+constexpr int kSmallChunks = 8;
+static_assert(kChunk == kChunk8, "one count of chunks for both");
+
+struct SmallTable {
+    Entry t[kSmallTable];
+    float *step[kSmallTable];
+    uint32_t numel[kSmallTable];
+    int32_t first[kSmallTable + 1];
+    int32_t count;
+};
+static_assert(sizeof(SmallTable) + sizeof(Scalars) + sizeof(Betas) + 32 <= 4096, "kernel arguments");
+
+template <class T, int BITS>
+__global__ __launch_bounds__(kSmallThreads) void adamw_small_kernel(SmallTable t, Scalars p, Betas b)
+{
+    __shared__ double part[kSmallThreads / 64];
+    __shared__ double grad;
+    __shared__ Factors factors[kSmallTable];
+    const int chunks = t.first[t.count];
+    const int team = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kThreads), mine = threadIdx.x % kThreads;
+    double acc = 0.0;
+    if (p.max_norm > 0.0)
+        for (int chunk = team; chunk < chunks; chunk += kSmallThreads / kThreads) {
+            const int k = __builtin_amdgcn_readfirstlane(tensor_of<kSmallTable>(t.first, t.count, chunk));
+            const int at = (chunk - t.first[k]) * kChunk + mine * 8;
+            const auto w = load_words<T, 8>((const T *)t.t[k].grad + at, (int)t.numel[k] - at);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc += (double)w[j] * (double)w[j];
+        }
+    acc = group_sum(acc, part, kSmallThreads / 64);
+    if (threadIdx.x == 0) grad = grad_factor(p, acc);
+    __syncthreads();
+    if ((int)threadIdx.x < t.count) factors[threadIdx.x] = factors_of(p, t.step[threadIdx.x], grad);
+    __syncthreads();
+    for (int chunk = team; chunk < chunks; chunk += kSmallThreads / kThreads) {
+        const int k = __builtin_amdgcn_readfirstlane(tensor_of<kSmallTable>(t.first, t.count, chunk));
+        const Factors f = factors[k];
+        if (f.skip) return;
+        const int at = (chunk - t.first[k]) * kChunk, left = (int)t.numel[k] - at;
+        if constexpr (BITS == 32) {
+            if (left >= kChunk)
+                update_chunk<true, false, T>(t.t[k], at + mine * 4, 0, b, f);
+            else
+                update_chunk<false, false, T>(t.t[k], at + mine * 4, left - mine * 4, b, f);
+        } else {
+            if (left >= kChunk8)
+                update_chunk8<true, false, T>(t.t[k], at + mine * 8, 0, at + mine * 8, b, f);
+            else if (mine * 8 / kBlock * kBlock < left)
+                update_chunk8<false, false, T>(t.t[k], at + mine * 8, left - mine * 8, at + mine * 8, b, f);
+        }
     }
 }
 
@@ -566,12 +645,56 @@ extern "C" int sv3d_grad_square_sums(const sv3d_adamw_tensor *tensors, int32_t n
     });
 }
 
-extern "C" int sv3d_adamw_workspace(int32_t num_tensors, size_t *bytes)
+extern "C" int sv3d_adamw_workspace(const sv3d_adamw_params *p, const sv3d_adamw_tensor *tensors, int32_t num_tensors,
+                                    size_t *bytes)
 {
-    if (num_tensors < 0 || !bytes) return SV3D_ERR_INVALID_ARG;
-    *bytes = (size_t)num_tensors * sizeof(Factors);
+    if (!p || num_tensors < 0 || !bytes) return SV3D_ERR_INVALID_ARG;
+    int32_t sums = 0;
+    if (p->max_norm > 0.0 && !p->square_sums)
+        if (const int st = sv3d_grad_square_sums_count(tensors, num_tensors, &sums)) return st;
+    *bytes = (size_t)num_tensors * sizeof(Factors) + (size_t)sums * sizeof(double);
     return SV3D_OK;
 }
+
+namespace {
+
+// Whether the call is the small kernel's: one type and kind of moments, few elements, and no norm from elsewhere.  Where that
+// kernel has work for its four teams once or twice, it takes the time of one launch in place of three (5136 elements,
+// clipped, 15.3 -> 7.8 us with the call's host time; at 16 chunks 15.4 and 13.4 us, not clipped 11.3 and 11.6).
+bool small_call(const sv3d_adamw_params *p, const sv3d_adamw_tensor *tensors, int32_t n)
+{
+    if (n > kSmallTable || p->square_sums) return false;
+    int64_t chunks = 0;
+    for (int32_t i = 0; i < n; ++i) {
+        if (tensors[i].type != tensors[0].type || tensors[i].state_bits != tensors[0].state_bits) return false;
+        if (tensors[i].numel > kSmallChunks * kChunk) return false;
+        chunks += (tensors[i].numel + kChunk - 1) / kChunk;
+    }
+    return chunks <= kSmallChunks;
+}
+
+int small_step(const Scalars &scalars, const Betas &b, const sv3d_adamw_tensor *tensors, int32_t n, hipStream_t stream)
+{
+    SmallTable t;
+    t.count = n;
+    t.first[0] = 0;
+    for (int i = 0; i < n; ++i) {
+        const sv3d_adamw_tensor &s = tensors[i];
+        t.t[i] = {s.param, s.grad, s.exp_avg, s.exp_avg_sq, s.scales};
+        t.step[i] = s.step;
+        t.numel[i] = (uint32_t)s.numel;
+        t.first[i + 1] = t.first[i] + (int32_t)((s.numel + kChunk - 1) / kChunk);
+    }
+    return for_each_type([&](auto *T, int32_t type) {
+        using E = std::remove_pointer_t<decltype(T)>;
+        if (type != tensors[0].type) return (int)SV3D_OK;
+        const auto kernel = tensors[0].state_bits == 32 ? adamw_small_kernel<E, 32> : adamw_small_kernel<E, 8>;
+        hipLaunchKernelGGL(kernel, dim3(1), dim3(kSmallThreads), 0, stream, t, scalars, b);
+        return launch_status();
+    });
+}
+
+}  // namespace
 
 extern "C" int sv3d_adamw_step(const sv3d_adamw_params *p, const sv3d_adamw_tensor *tensors, int32_t num_tensors,
                                void *workspace, size_t workspace_bytes, void *stream)
@@ -579,22 +702,35 @@ extern "C" int sv3d_adamw_step(const sv3d_adamw_params *p, const sv3d_adamw_tens
     if (!p) return SV3D_ERR_INVALID_ARG;
     if (const int st = check(tensors, num_tensors, false)) return st;
     if (!(p->beta1 >= 0.0 && p->beta1 < 1.0 && p->beta2 >= 0.0 && p->beta2 < 1.0 && p->eps >= 0.0)) return SV3D_ERR_INVALID_ARG;
-    if (p->square_sums && (p->num_square_sums < 0 || !(p->max_norm >= 0.0))) return SV3D_ERR_INVALID_ARG;
+    if (!(p->max_norm >= 0.0) || p->num_square_sums < 0) return SV3D_ERR_INVALID_ARG;
     if (num_tensors == 0) return SV3D_OK;
+    size_t need = 0;
+    if (const int st = sv3d_adamw_workspace(p, tensors, num_tensors, &need)) return st;
     if (!workspace || !aligned(workspace, 16)) return SV3D_ERR_INVALID_ARG;
-    if (workspace_bytes < (size_t)num_tensors * sizeof(Factors)) return SV3D_ERR_WORKSPACE;
+    if (workspace_bytes < need) return SV3D_ERR_WORKSPACE;
+    const Scalars scalars = {p->lr,         log(p->beta1), log(p->beta2), p->weight_decay, p->max_norm, p->lr_device,
+                             p->grad_scale, p->found_inf,  p->total_norm, p->seed,         p->maximize};
+    const Betas b = {(float)p->beta1, (float)(1.0 - p->beta1), (float)p->beta2, (float)(1.0 - p->beta2),
+                     (float)(p->eps > 0x1p-63 ? p->eps : 0x1p-63)};
+    if (small_call(p, tensors, num_tensors)) return small_step(scalars, b, tensors, num_tensors, (hipStream_t)stream);
     Factors *factors = (Factors *)workspace;
+    const bool clip = p->max_norm > 0.0, read_before = clip && !p->square_sums;
+    const double *sums = p->square_sums;
+    int32_t num_sums = clip ? p->num_square_sums : 0;
+    if (read_before) {
+        num_sums = (int32_t)((need - num_tensors * sizeof(Factors)) / sizeof(double));
+        double *own = (double *)(factors + num_tensors);
+        if (const int st = sv3d_grad_square_sums(tensors, num_tensors, own, num_sums, stream)) return st;
+        sums = own;
+    }
     for (int32_t base = 0; base < num_tensors; base += kSteps) {
         StepTable s;
         s.base = base;
         s.count = num_tensors - base < kSteps ? num_tensors - base : kSteps;
         for (int i = 0; i < s.count; ++i) s.step[i] = tensors[base + i].step;
-        hipLaunchKernelGGL(adamw_factors_kernel, dim3(1), dim3(kThreads), 0, (hipStream_t)stream, s, *p, factors);
+        hipLaunchKernelGGL(adamw_factors_kernel, dim3(1), dim3(kThreads), 0, (hipStream_t)stream, s, scalars, sums, num_sums, factors);
         if (const int st = launch_status()) return st;
     }
-    const Betas b = {(float)p->beta1, (float)(1.0 - p->beta1), (float)p->beta2, (float)(1.0 - p->beta2),
-                     (float)(p->eps > 0x1p-63 ? p->eps : 0x1p-63)};
-    const bool read_before = p->square_sums != nullptr;
     return for_each_type([&](auto *T, int32_t type) {
         using E = std::remove_pointer_t<decltype(T)>;
         for (int32_t bits : {32, 8}) {

@@ -446,16 +446,18 @@ Tensor adamw_step_gpu(TensorList params, TensorList grads, TensorList exp_avgs, 
     p.maximize = maximize ? 1 : 0;
     p.seed = (uint32_t)seed;
     Tensor norm = at::empty({}, ref.options().dtype(at::kFloat));
-    if (given(square_sums)) {
+    if (max_norm > 0.0) p.total_norm = norm.data_ptr<float>();
+    Tensor none;
+    if (max_norm > 0.0 && given(square_sums)) {
         TORCH_CHECK_VALUE(square_sums->scalar_type() == at::kDouble && square_sums->is_contiguous() && square_sums->dim() == 1,
                           "square_sums must be what grad_square_sums returns");
         same_device(ref, *square_sums, "square_sums");
-        p.square_sums = square_sums->numel() > 0 ? square_sums->data_ptr<double>() : nullptr;
+        if (square_sums->numel() == 0) none = at::empty({1}, square_sums->options());       // the norm of nothing
+        p.square_sums = none.defined() ? none.data_ptr<double>() : square_sums->data_ptr<double>();
         p.num_square_sums = (int32_t)square_sums->numel();
-        p.total_norm = norm.data_ptr<float>();
     }
     size_t bytes = 0;
-    check_status(sv3d_adamw_workspace((int32_t)list.size(), &bytes), "sv3d_adamw_workspace");
+    check_status(sv3d_adamw_workspace(&p, list.data(), (int32_t)list.size(), &bytes), "sv3d_adamw_workspace");
     Tensor ws = at::empty({(int64_t)bytes}, ref.options().dtype(at::kByte));
     check_status(sv3d_adamw_step(&p, list.data(), (int32_t)list.size(), ws.data_ptr(), bytes, L.stream), "sv3d_adamw_step");
     // a graph that saved a weight for its backward has to see that the weight is another one now

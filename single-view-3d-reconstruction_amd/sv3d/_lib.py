@@ -133,7 +133,7 @@ def lib():
         L.sv3d_layer_norm_backward.argtypes = [lp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
         L.sv3d_grad_square_sums_count.argtypes = [at, i32, ctypes.POINTER(i32)]
         L.sv3d_grad_square_sums.argtypes = [at, i32, vp, i32, vp]
-        L.sv3d_adamw_workspace.argtypes = [i32, ctypes.POINTER(sz)]
+        L.sv3d_adamw_workspace.argtypes = [ctypes.POINTER(AdamWParams), at, i32, ctypes.POINTER(sz)]
         L.sv3d_adamw_step.argtypes = [ctypes.POINTER(AdamWParams), at, i32, vp, sz, vp]
         L.sv3d_moment_values.argtypes = [vp, vp, vp, i64, vp, vp, vp]
         mp = ctypes.POINTER(MeshInput)

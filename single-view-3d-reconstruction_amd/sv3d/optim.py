@@ -36,8 +36,6 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, scales=None, lr=1
     if clip and not max_norm > 0:
         raise ValueError("max_norm must not be negative or NaN, got %r" % (max_norm,))
     with torch.no_grad():
-        if clip and square_sums is None:
-            square_sums = call("grad_square_sums", grads)
         tensor_lr = lr if torch.is_tensor(lr) else None
         norm = call("adamw_step", params, grads, exp_avgs, exp_avg_sqs, scales if scales is not None else [], steps, tensor_lr,
                                grad_scale, found_inf, square_sums if clip else None, 0.0 if tensor_lr is not None else lr,

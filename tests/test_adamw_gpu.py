@@ -536,3 +536,27 @@ def test_more_elements_than_32_bits_count():
     assert_codes(to.decode(m[mid: mid + 300].cpu(), bytes_mid[:, 0], to.FIRST), want["m"], want["e_m"], bytes_mid[:, 0], to.FIRST,
                  x // 65536, "exp_avg")
     assert not p[300:1000].any() and not p[mid + 300: mid + 1000].any() and not m[far - 1000: far].any()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+def test_small_calls_give_the_bits_of_large_ones(bits, t):
+    """A few thousand elements take one workgroup and one launch; among many others they take the general way."""
+    few = [1, 2048, 130, 3001, 0, 2049]
+    small, large = Set(few, t, bits, seed=1, offset=1), Set(few + [60000], t, bits, seed=1, offset=1)
+    for k in range(3):
+        a = small.step(max_norm=1e9, grad_scale=torch.tensor(2.0).cuda(), found_inf=torch.tensor(float(k == 1)).cuda())
+        b = large.step(max_norm=1e9, grad_scale=torch.tensor(2.0).cuda(), found_inf=torch.tensor(float(k == 1)).cuda())
+        assert float(a) <= float(b)
+        for x, y in ((small.p, large.p), (small.m, large.m), (small.v, large.v), (small.e, large.e), (small.steps, large.steps)):
+            assert all(torch.equal(i, j) for i, j in zip(x, y)), k
+    small.assert_untouched_around()
+
+
+def test_empty_tensors_and_a_norm_of_nothing():
+    s = Set([0, 0])
+    assert float(s.step(max_norm=1.0)) == 0.0 and all(float(t) == 4.0 for t in s.steps)
+    sums = optim.grad_square_sums(s.g)
+    assert sums.numel() == 0 and float(s.step(max_norm=1.0, square_sums=sums)) == 0.0
+    s = Set([0, 5, 0])
+    check_step(s, max_norm=0.1)

@@ -267,8 +267,13 @@ def test_abi_square_sums_and_moment_values_refuse():
     assert lib.sv3d_moment_values(SOME, SOME, SOME, -1, SOME, SOME, None) == INVALID
     assert lib.sv3d_moment_values(SOME, None, SOME, 5, SOME, SOME, None) == INVALID
     assert lib.sv3d_moment_values(None, None, None, 0, None, None, None) == 0
-    count = ctypes.c_size_t()
-    assert lib.sv3d_adamw_workspace(-1, ctypes.byref(count)) == INVALID
+    count, p = ctypes.c_size_t(), L.AdamWParams(beta1=0.9, beta2=0.9, max_norm=1.0)
+    assert lib.sv3d_adamw_workspace(ctypes.byref(p), arr, -1, ctypes.byref(count)) == INVALID
+    assert lib.sv3d_adamw_workspace(ctypes.byref(p), None, 2, ctypes.byref(count)) == INVALID
+    assert lib.sv3d_adamw_workspace(ctypes.byref(p), arr, 2, ctypes.byref(count)) == 0
+    clipped = count.value
+    p.max_norm = 0.0
+    assert lib.sv3d_adamw_workspace(ctypes.byref(p), arr, 2, ctypes.byref(count)) == 0 and clipped - count.value == 8 * n.value
     assert lib.sv3d_adamw_step(ctypes.byref(L.AdamWParams(beta1=0.9, beta2=0.9)), None, 0, None, 0, None) == 0
 
 
