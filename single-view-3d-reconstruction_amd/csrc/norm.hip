@@ -45,6 +45,15 @@ __device__ inline float row_sum(float v, float *part)
     return v;
 }
 
+template <int V>
+__device__ inline float sum_of(const float *v)
+{
+    float s = v[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j) s += v[j];
+    return s;
+}
+
 // A row's packs.  Where the row's end cuts one, the pack that ends with the row is loaded in its place and what it
 // repeats is dropped when the values are used (drop_end): put together from single elements, a pack would have to
 // be waited for where it is loaded, and no load of the next row would be on its way during the work on this one.  Rows of
@@ -156,39 +165,37 @@ __global__ __launch_bounds__(kGroup<G>) void layer_norm_forward_kernel(
 // ---- rows beyond registers: a workgroup per row, which it reads three times ----------------------------
 constexpr int kLong = 1024;
 
-template <class X>
-__device__ inline float param(const void *p, bool f32, float missing, int c)
-{
-    return !p ? missing : f32 ? ((const float *)p)[c] : to_float(((const X *)p)[c]);
-}
-
 template <class X, class Y>
 __global__ __launch_bounds__(kLong) void layer_norm_forward_long_kernel(
     const X *__restrict__ x, const void *__restrict__ weight, const void *__restrict__ bias, int params_f32, int cols,
     int64_t rows, int64_t x_stride, float eps, Y *__restrict__ y, float *__restrict__ mean, float *__restrict__ rstd)
 {
+    constexpr int V = kPack<X>;
     __shared__ float part[2][kLong / 64];
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const X *xr = x + row * x_stride;
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int c0 = threadIdx.x; c0 < cols; c0 += 4 * kLong)
+        float s[V] = {};
+        for (int c = threadIdx.x * V; c < cols; c += kLong * V) {
+            const auto w = load_words<X, V>(xr + c, cols - c);
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (c0 + u * kLong < cols) s[u] += to_float(xr[c0 + u * kLong]);
-        const float mu = row_sum<kLong>((s[0] + s[1]) + (s[2] + s[3]), part[0]) / (float)cols;
-        float q[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int c0 = threadIdx.x; c0 < cols; c0 += 4 * kLong)
+            for (int j = 0; j < V; ++j) s[j] += w[j];           // zero behind the row's end
+        }
+        const float mu = row_sum<kLong>(sum_of<V>(s), part[0]) / (float)cols;
+        float q[V] = {};
+        for (int c = threadIdx.x * V; c < cols; c += kLong * V) {
+            const auto w = load_words<X, V>(xr + c, cols - c);
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (c0 + u * kLong < cols) {
-                    const float d = to_float(xr[c0 + u * kLong]) - mu;
-                    q[u] += d * d;
-                }
-        const float r = 1.f / sqrtf(row_sum<kLong>((q[0] + q[1]) + (q[2] + q[3]), part[1]) / (float)cols + eps);
-        Y *yr = y + row * cols;
-        for (int c = threadIdx.x; c < cols; c += kLong) {
-            const float w = param<X>(weight, params_f32, 1.f, c), b = param<X>(bias, params_f32, 0.f, c);
-            yr[c] = from_float<Y>((to_float(xr[c]) - mu) * r * w + b);
+            for (int j = 0; j < V; ++j) q[j] += c + j < cols ? (w[j] - mu) * (w[j] - mu) : 0.f;
+        }
+        const float r = 1.f / sqrtf(row_sum<kLong>(sum_of<V>(q), part[1]) / (float)cols + eps);
+        for (int c = threadIdx.x * V; c < cols; c += kLong * V) {
+            const auto v = load_words<X, V>(xr + c, cols - c);
+            float w[V], b[V];
+            load_params<X, V, true>(weight, params_f32, 1.f, c, cols - c, w);
+            load_params<X, V, true>(bias, params_f32, 0.f, c, cols - c, b);
+#pragma unroll
+            for (int j = 0; j < V; ++j) w[j] = (v[j] - mu) * r * w[j] + b[j];
+            store_pack<Y, V>(y + row * cols + c, w, cols - c);
         }
         if (threadIdx.x == 0) {
             if (mean) mean[row] = mu;
@@ -361,49 +368,65 @@ __global__ __launch_bounds__(kLong) void layer_norm_dx_long_kernel(
     const X *__restrict__ x, const Y *__restrict__ dy, const void *__restrict__ weight, int params_f32, int cols, int64_t rows,
     const float *__restrict__ mean, const float *__restrict__ rstd, int64_t x_stride, int64_t dy_stride, X *__restrict__ dx)
 {
+    constexpr int V = kPack<X>;
     __shared__ float part[2][kLong / 64];
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const X *xr = x + row * x_stride;
         const Y *dr = dy + row * dy_stride;
         const float mu = mean[row], r = rstd[row];
-        float su[2] = {0.f, 0.f}, sh[2] = {0.f, 0.f};
-        for (int c0 = threadIdx.x; c0 < cols; c0 += 2 * kLong)
+        float su[V] = {}, sh[V] = {};
+        for (int c = threadIdx.x * V; c < cols; c += kLong * V) {
+            const auto v = load_words<X, V>(xr + c, cols - c);
+            const auto d = load_words<Y, V>(dr + c, cols - c);
+            float w[V];
+            load_params<X, V, true>(weight, params_f32, 1.f, c, cols - c, w);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int c = c0 + t * kLong;
-                if (c >= cols) break;
-                const float u = to_float(dr[c]) * param<X>(weight, params_f32, 1.f, c);
-                su[t] += u;
-                sh[t] += u * ((to_float(xr[c]) - mu) * r);
+            for (int j = 0; j < V; ++j) {
+                const float u = d[j] * w[j];                    // zero behind the row's end
+                su[j] += u;
+                sh[j] += u * ((v[j] - mu) * r);
             }
-        const float mu_u = row_sum<kLong>(su[0] + su[1], part[0]) / (float)cols;
-        const float mu_uh = row_sum<kLong>(sh[0] + sh[1], part[1]) / (float)cols;
-        X *o = dx + row * cols;
-        for (int c = threadIdx.x; c < cols; c += kLong) {
-            const float w = param<X>(weight, params_f32, 1.f, c);
-            o[c] = from_float<X>((to_float(dr[c]) * w - mu_u - (to_float(xr[c]) - mu) * r * mu_uh) * r);
+        }
+        const float mu_u = row_sum<kLong>(sum_of<V>(su), part[0]) / (float)cols;
+        const float mu_uh = row_sum<kLong>(sum_of<V>(sh), part[1]) / (float)cols;
+        for (int c = threadIdx.x * V; c < cols; c += kLong * V) {
+            const auto v = load_words<X, V>(xr + c, cols - c);
+            const auto d = load_words<Y, V>(dr + c, cols - c);
+            float w[V];
+            load_params<X, V, true>(weight, params_f32, 1.f, c, cols - c, w);
+#pragma unroll
+            for (int j = 0; j < V; ++j) w[j] = (d[j] * w[j] - mu_u - (v[j] - mu) * r * mu_uh) * r;
+            store_pack<X, V>(dx + row * cols + c, w, cols - c);
         }
     }
 }
 
-// dweight and dbias of such rows: a thread per column adds up a slice of the rows
-constexpr int kSlices = 64;
+// dweight and dbias of such rows: a thread for a few columns adds up a slice of the rows
+constexpr int kSlices = 64, kSliceColumns = 4;
 
 template <class X, class Y>
 __global__ __launch_bounds__(kThreads) void layer_norm_slices_kernel(
     const X *__restrict__ x, const Y *__restrict__ dy, const float *__restrict__ mean, const float *__restrict__ rstd,
     int64_t rows, int cols, int64_t x_stride, int64_t dy_stride, float *__restrict__ part)
 {
-    const int c = blockIdx.x * kThreads + threadIdx.x;
-    if (c >= cols) return;
-    float w = 0.f, b = 0.f;
+    constexpr int V = kSliceColumns;
+    const int c = (blockIdx.x * kThreads + threadIdx.x) * V, n = cols - c;
+    if (n <= 0) return;
+    float w[V] = {}, b[V] = {};
+#pragma unroll 4
     for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
-        const float d = to_float(dy[row * dy_stride + c]);
-        w += d * ((to_float(x[row * x_stride + c]) - mean[row]) * rstd[row]);
-        b += d;
+        const auto v = load_words<X, V>(x + row * x_stride + c, n);
+        const auto d = load_words<Y, V>(dy + row * dy_stride + c, n);
+        const float mu = mean[row], r = rstd[row];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            w[j] += d[j] * ((v[j] - mu) * r);
+            b[j] += d[j];
+        }
     }
-    part[(2 * (int64_t)blockIdx.y) * cols + c] = w;
-    part[(2 * (int64_t)blockIdx.y + 1) * cols + c] = b;
+    float *out = part + 2 * (int64_t)blockIdx.y * cols + c;
+    store_pack<float, V>(out, w, n);
+    store_pack<float, V>(out + cols, b, n);
 }
 
 // The sum over the `count` partial sums: 16 columns of one of the two gradients per workgroup, 64 threads each.
@@ -623,7 +646,7 @@ extern "C" int sv3d_layer_norm_backward(const sv3d_layer_norm_params *p, const v
                                            dim3(kLong), 0, s, (const X *)x, (const Y *)dy, weight, f32, cols, p->rows, mean,
                                            rstd, p->x_stride, p->dy_stride, (X *)dx);
                     if (part)
-                        hipLaunchKernelGGL((layer_norm_slices_kernel<X, Y>), dim3((cols + kThreads - 1) / kThreads, count),
+                        hipLaunchKernelGGL((layer_norm_slices_kernel<X, Y>), dim3((cols + kThreads * kSliceColumns - 1) / (kThreads * kSliceColumns), count),
                                            dim3(kThreads), 0, s, (const X *)x, (const Y *)dy, mean, rstd, p->rows, cols,
                                            p->x_stride, p->dy_stride, part);
                 }
