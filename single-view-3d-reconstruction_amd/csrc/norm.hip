@@ -19,7 +19,7 @@ template <class X>
 constexpr int kPack = 16 / (int)sizeof(X);
 
 template <int G>
-constexpr int kGroup = G > 256 ? G : 256;       // threads of the workgroup
+constexpr int kGroup = G > 64 ? G : 256;        // threads of the workgroup
 
 // Which of a workgroup's rows a thread works on: known to the whole wave (and kept in scalar registers, the row's
 // addresses with it) where a wave has no more than one.
@@ -461,9 +461,11 @@ int check(const sv3d_layer_norm_params *p)
     return SV3D_OK;
 }
 
-// Threads per row and packs per thread that hold `cols` columns, as a call f(G, K): the fewest threads that do with at
-// most two packs each up to 64 threads (rows that share a wave or have one to themselves add up without a barrier), then
-// 256 threads, then 1024; f(0, 0) beyond.
+// Threads per row and packs per thread that hold `cols` columns, as a call f(G, K): the fewest threads that do with one
+// pack each, but two before a row needs more than a wave (with a wave to itself it is added up without a barrier: 32768 x
+// 1024 bf16 24.1 us, 25.9 with one pack in 128 threads), and more than one beyond 1024 threads; f(0, 0) beyond those.
+// With one pack a thread needs no more than 64 registers and a CU holds 2048 of them: 16384 x 4096 bf16 53.3 us with two
+// packs in 256 threads, 49.8 with one in 512.
 template <int G_, int K_>
 struct Shape {
     static constexpr int G = G_, K = K_;
@@ -479,8 +481,8 @@ int with_shape(int64_t cols, F f)
     if (packs <= 64) return f(Shape<64, 1>());
     if (packs <= 128) return f(Shape<64, 2>());
     if (packs <= 256) return f(Shape<256, 1>());
-    if (packs <= 512) return f(Shape<256, 2>());
-    if (packs <= 1024) return f(Shape<256, 4>());
+    if (packs <= 512) return f(Shape<512, 1>());
+    if (packs <= 1024) return f(Shape<1024, 1>());
     if (packs <= 2048) return f(Shape<1024, 2>());
     if constexpr (kPack<X> == 4)
         if (packs <= 4096) return f(Shape<1024, 4>());
@@ -525,9 +527,9 @@ int with_ends(bool ends, bool stream, F f)
 
 // A workgroup for each set of rows, but no more than the device holds at once: more rows are taken in turn, with the
 // weights in registers and the next row's load on its way.
-uint32_t persistent_groups(int64_t rows, int rows_per_group, int threads)
+uint32_t persistent_groups(int64_t rows, int rows_per_group, int threads, int per_cu = 2048)
 {
-    const int64_t want = (rows + rows_per_group - 1) / rows_per_group, fit = 256 * (2048 / threads);
+    const int64_t want = (rows + rows_per_group - 1) / rows_per_group, fit = 256 * (per_cu / threads);
     return (uint32_t)(want < fit ? want : fit);
 }
 
@@ -590,7 +592,8 @@ extern "C" int sv3d_layer_norm_forward(const sv3d_layer_norm_params *p, const vo
             else
                 with_ends(cols % kPack<X> != 0, p->rows * cols * (int64_t)(sizeof(X) + sizeof(Y)) >= kLastCache, [&](auto ends, auto past) {
                     hipLaunchKernelGGL((layer_norm_forward_kernel<X, Y, G, K, decltype(ends)::value, decltype(past)::value>),
-                                       dim3(persistent_groups(p->rows, kGroup<G> / G, kGroup<G>)), dim3(kGroup<G>), 0,
+                                       dim3(persistent_groups(p->rows, kGroup<G> / G, kGroup<G>, G == 1024 && K > 1 ? 1024 : 2048)),
+                                       dim3(kGroup<G>), 0,
                                        (hipStream_t)stream, (const X *)x, weight, bias, f32, cols, p->rows, p->x_stride, p->eps,
                                        (Y *)y, mean, rstd);
                     return 0;
