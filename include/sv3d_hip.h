@@ -350,11 +350,11 @@ typedef struct sv3d_layer_norm_params {
 } sv3d_layer_norm_params;
 
 /* `weight`, `bias` may be NULL (1 and 0), `mean`, `rstd` [rows] too (nobody will call the backward).
- * y is contiguous. */
+ * y is contiguous and overlaps none of the inputs; addresses are multiples of their element's size. */
 int sv3d_layer_norm_forward(const sv3d_layer_norm_params *p, const void *x, const void *weight, const void *bias,
                             void *y, float *mean, float *rstd, void *stream);
 
-/* Gradients of the call above; each of dx (contiguous), dweight, dbias may be NULL.  dweight and dbias
+/* Gradients of the call above; each of dx (contiguous, not dy's or x's memory), dweight, dbias may be NULL.  dweight and dbias
  * are sums over the rows in an order that the sizes fix; they need `workspace`, at least
  * sv3d_layer_norm_workspace() bytes, 16-byte aligned, whose content does not matter. */
 int sv3d_layer_norm_workspace(const sv3d_layer_norm_params *p, size_t *bytes);

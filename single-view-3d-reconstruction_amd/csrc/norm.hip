@@ -579,6 +579,9 @@ extern "C" int sv3d_layer_norm_forward(const sv3d_layer_norm_params *p, const vo
     if (const int st = check(p)) return st;
     if (p->rows == 0) return SV3D_OK;
     if (!x || !y) return SV3D_ERR_INVALID_ARG;
+    if (!aligned(x, type_bytes(p->x_type)) || !aligned(y, type_bytes(p->y_type)) || !aligned(weight, type_bytes(p->param_type)) ||
+        !aligned(bias, type_bytes(p->param_type)) || !aligned(mean, 4) || !aligned(rstd, 4))
+        return SV3D_ERR_INVALID_ARG;
     return with_xy(p, [&](auto *xt, auto *yt) {
         using X = std::remove_pointer_t<decltype(xt)>;
         using Y = std::remove_pointer_t<decltype(yt)>;
@@ -619,6 +622,10 @@ extern "C" int sv3d_layer_norm_backward(const sv3d_layer_norm_params *p, const v
     if (const int st = check(p)) return st;
     if (p->dy_stride < 0) return SV3D_ERR_INVALID_ARG;
     if (p->rows > 0 && (!x || !dy || !mean || !rstd)) return SV3D_ERR_INVALID_ARG;
+    if (!aligned(x, type_bytes(p->x_type)) || !aligned(dy, type_bytes(p->y_type)) || !aligned(dx, type_bytes(p->x_type)) ||
+        !aligned(weight, type_bytes(p->param_type)) || !aligned(dweight, type_bytes(p->param_type)) ||
+        !aligned(dbias, type_bytes(p->param_type)) || !aligned(mean, 4) || !aligned(rstd, 4))
+        return SV3D_ERR_INVALID_ARG;
     const bool params = dweight || dbias;
     if (params && p->rows > 0) {
         size_t need = 0;

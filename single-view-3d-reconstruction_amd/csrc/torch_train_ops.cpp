@@ -262,6 +262,8 @@ Tensor layer_norm_autograd(const Tensor &x, IntList shape, const optional<Tensor
                            double eps, bool f32_out)
 {
     const Tensor w = given(weight) ? *weight : Tensor(), b = given(bias) ? *bias : Tensor();
+    for (const Tensor *t : {&x, &w, &b})
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), "sv3d::layer_norm has no forward-mode derivative");
     if (!torch::autograd::compute_requires_grad(x, w, b)) {
         // no gradient will be asked for: without the statistics of the rows
         at::AutoDispatchBelowADInplaceOrView guard;

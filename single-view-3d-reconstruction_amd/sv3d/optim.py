@@ -80,6 +80,11 @@ class AdamW(torch.optim.Optimizer):
         self.total_norm = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize))
 
+    _own = ("max_norm", "state_bits", "min_8bit_size", "seed", "total_norm")
+
+    def __getstate__(self):
+        return {**super().__getstate__(), **{name: getattr(self, name) for name in self._own}}
+
     def _new_state(self, p):
         if p.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("sv3d.optim.AdamW makes its state on a tensor's first step, which must come before the capture")
@@ -119,7 +124,7 @@ class AdamW(torch.optim.Optimizer):
                 scales = [s.get("scales", none) for s in states]
             work.append((group, params, [p.grad for p in params], states, scales))
         sums = None
-        if self.max_norm > 0 and work:
+        if self.max_norm > 0 and len(work) > 1:         # one norm over all groups
             sums = grad_square_sums([g for w in work for g in w[2]])
         for group, params, grads, states, scales in work:
             norm = adamw_step(params, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],

@@ -175,6 +175,21 @@ def test_state_dict_of_8_bit_moments_survives_loading_into_a_16_bit_model():
         assert b.state[q][name].data_ptr() != value.data_ptr()
 
 
+def test_optimizer_can_be_copied_and_pickled():
+    import copy
+    import pickle
+    a = optim.AdamW([torch.nn.Parameter(torch.zeros(3))], lr=0.5, max_norm=0.25, state_bits=8, min_8bit_size=7, seed=11)
+    for b in (copy.deepcopy(a), pickle.loads(pickle.dumps(a))):
+        assert (b.max_norm, b.state_bits, b.min_8bit_size, b.seed, b.param_groups[0]["lr"]) == (0.25, 8, 7, 11, 0.5)
+
+
+def test_layer_norm_refuses_forward_mode_derivatives():
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            norm.layer_norm(fwd.make_dual(meta(2, 8), meta(2, 8)), 8)
+
+
 def test_convert_layer_norm_keeps_parameters_and_leaves_subclasses_alone():
     class Own(torch.nn.LayerNorm):
         pass
@@ -212,6 +227,11 @@ def test_abi_layer_norm_refuses(kw, x, status):
 
 def test_abi_layer_norm_workspace_and_empty_calls():
     lib = L.lib()
+    p = norm_params()
+    for odd in range(5):                                # addresses off their element's size
+        a = [SOME + 1 if i == odd else SOME for i in range(5)]
+        assert lib.sv3d_layer_norm_forward(ctypes.byref(p), a[0], a[1], a[2], a[3], a[4], SOME, None) == INVALID
+        assert lib.sv3d_layer_norm_backward(ctypes.byref(p), a[0], a[1], a[2], SOME, SOME, a[3], a[4], None, SOME, 1 << 30, None) == INVALID
     assert lib.sv3d_layer_norm_forward(None, SOME, None, None, SOME, None, None, None) == INVALID
     p, n = norm_params(), ctypes.c_size_t()
     assert lib.sv3d_layer_norm_workspace(ctypes.byref(p), None) == INVALID
