@@ -116,14 +116,15 @@ __device__ inline double grad_factor(const Scalars &p, double square_sum)
 }
 
 // Takes a tensor's step count forward.  In double: beta^t close to 1 is subtracted from 1.
-__device__ inline Factors factors_of(const Scalars &p, float *step, double grad)
+// `grad` is left to the caller.
+__device__ inline Factors factors_of(const Scalars &p, float *step)
 {
     const int32_t skip = p.found_inf && *p.found_inf != 0.f;
     const double lr = p.lr_device ? (double)*p.lr_device : p.lr;
     const float n = *step + 1.f;
     if (!skip) *step = n;
     Factors f;
-    f.grad = (float)grad;
+    f.grad = 0.f;
     f.decay = (float)(1.0 - lr * p.weight_decay);
     f.rate = (float)(lr / -expm1((double)n * p.log_b1));
     f.root = (float)(1.0 / sqrt(-expm1((double)n * p.log_b2)));
@@ -140,18 +141,32 @@ struct StepTable {
 };
 static_assert(sizeof(StepTable) + sizeof(Scalars) + 32 <= 4096, "kernel arguments");
 
-// One workgroup: the factors of up to kSteps tensors.
+// One workgroup: the factors of up to kSteps tensors.  All that does not depend on the norm goes before the wait for its
+// partial sums, whose loads go out together (14 M weights, clipped: 75.9 -> 74.8 us).
 __global__ __launch_bounds__(kThreads) void adamw_factors_kernel(StepTable t, Scalars p, const double *__restrict__ sums,
                                                                  int num_sums, Factors *__restrict__ out)
 {
     __shared__ double part[kThreads / 64];
     __shared__ double grad;
-    double acc = 0.0;
-    for (int i = threadIdx.x; i < num_sums; i += kThreads) acc += sums[i];
+    constexpr int U = kSumGroups / kThreads;
+    double sum[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) sum[u] = u * kThreads + (int)threadIdx.x < num_sums ? sums[u * kThreads + threadIdx.x] : 0.0;
+    Factors mine;
+    if ((int)threadIdx.x < t.count) mine = factors_of(p, t.step[threadIdx.x]);
+    double acc = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    static_assert(U == 4, "what one launch of sums leaves");
+    for (int i = kSumGroups + threadIdx.x; i < num_sums; i += kThreads) acc += sums[i];
     acc = group_sum(acc, part, kThreads / 64);
     if (threadIdx.x == 0) grad = grad_factor(p, acc);
     __syncthreads();
-    for (int i = threadIdx.x; i < t.count; i += kThreads) out[t.base + i] = factors_of(p, t.step[i], grad);
+    mine.grad = (float)grad;
+    if ((int)threadIdx.x < t.count) out[t.base + threadIdx.x] = mine;
+    for (int i = kThreads + threadIdx.x; i < t.count; i += kThreads) {
+        Factors f = factors_of(p, t.step[i]);
+        f.grad = (float)grad;
+        out[t.base + i] = f;
+    }
 }
 
 // ---- 8-bit moments -----------------------------------------------------------------------------------
@@ -482,15 +497,15 @@ __global__ __launch_bounds__(kSmallThreads) void adamw_small_kernel(SmallTable t
 #pragma unroll
             for (int j = 0; j < 8; ++j) acc += (double)w[j] * (double)w[j];
         }
+    if ((int)threadIdx.x < t.count) factors[threadIdx.x] = factors_of(p, t.step[threadIdx.x]);
     acc = group_sum(acc, part, kSmallThreads / 64);
     if (threadIdx.x == 0) grad = grad_factor(p, acc);
     __syncthreads();
-    if ((int)threadIdx.x < t.count) factors[threadIdx.x] = factors_of(p, t.step[threadIdx.x], grad);
-    __syncthreads();
     for (int chunk = team; chunk < chunks; chunk += kSmallThreads / kThreads) {
         const int k = __builtin_amdgcn_readfirstlane(tensor_of<kSmallTable>(t.first, t.count, chunk));
-        const Factors f = factors[k];
+        Factors f = factors[k];
         if (f.skip) return;
+        f.grad = (float)grad;
         const int at = (chunk - t.first[k]) * kChunk, left = (int)t.numel[k] - at;
         if constexpr (BITS == 32) {
             if (left >= kChunk)
