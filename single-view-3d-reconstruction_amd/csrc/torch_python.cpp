@@ -1,9 +1,9 @@
 // Python's direct way to the operators that are called with long lists or for little work (torch_train_ops.cpp): the module
-// sv3d._call.  Its functions take the operators' arguments by position, turn them into C++ values (a list of 70 tensors
-// costs 2 us here, 15 us through the generic arguments of torch.ops) and call the operator through the dispatcher, so that
-// everything that works on operators (autograd, shape-only tensors, tracing modes) still sees them.  Arguments that are
-// not plain tensors (subclasses with their own __torch_function__, or an active mode of that kind) are answered with
-// NotImplemented: the caller then goes through torch.ops.
+// sv3d._call.  Its functions take the operators' arguments by position, turn them into C++ values (an optimizer step on five
+// lists of 72 shape-only tensors took 71 us this way, 96 us through the generic arguments of torch.ops) and call the operator
+// through the dispatcher, so that everything that works on operators (autograd, shape-only tensors, tracing modes) still
+// sees them.  Arguments that are not plain tensors (subclasses with their own __torch_function__, or an active mode of that
+// kind) are answered with NotImplemented: the caller then goes through torch.ops.
 #include <Python.h>
 
 #include <torch/csrc/Exceptions.h>

@@ -137,12 +137,22 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """As every optimizer's; the moments keep their own types (8-bit codes or float32) whatever their weight's."""
+        """As every optimizer's, also from `torch.optim.Adam`'s and `AdamW`'s.  8-bit codes stay what they are, moments of
+        any other type become float32 in their weight's strides, whatever the weight's type; step counts and a
+        learning rate that is a tensor go to the weights' device."""
         kept = state_dict["state"]
         super().load_state_dict(state_dict)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, params):
             for name, value in kept.get(i, {}).items():
-                if torch.is_tensor(value):
-                    self.state[p][name] = value.detach().to(device=p.device, copy=True)
+                if name == "step":
+                    value = torch.as_tensor(value, dtype=torch.float32).detach().to(device=p.device, copy=True)
+                elif name in ("exp_avg", "exp_avg_sq") and value.dtype != torch.uint8 and value.shape == p.shape:
+                    value = torch.empty_like(p, dtype=torch.float32, requires_grad=False).copy_(value.detach())
+                elif torch.is_tensor(value):
+                    value = value.detach().to(device=p.device, copy=True)
+                self.state[p][name] = value
+        for group in self.param_groups:
+            if torch.is_tensor(group["lr"]) and group["params"]:
+                group["lr"] = group["lr"].detach().to(device=group["params"][0].device, dtype=torch.float32, copy=True)

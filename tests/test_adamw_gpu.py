@@ -296,6 +296,23 @@ def test_the_same_memory_twice_is_refused():
         optim.adamw_step(s.p, [s.g[0], s.g[1].cpu()], s.m, s.v, s.steps, **HYPER)
 
 
+def test_gradients_may_be_shared_but_lie_nowhere_else():
+    s = Set([300, 300])
+    before = [[x.clone() for x in list_] for list_ in (s.p, s.m, s.v, s.steps)]
+    for g in ([s.p[0], s.g[1]], [s.g[0], s.m[0]], [s.g[0], s.around[0][0][65:365]]):
+        with pytest.raises(ValueError):
+            optim.adamw_step(s.p, g, s.m, s.v, s.steps, **HYPER)
+    for list_, kept in zip((s.p, s.m, s.v, s.steps), before):
+        assert all(torch.equal(x, y) for x, y in zip(list_, kept))
+    twice = Set([300, 300])
+    twice.g[1].copy_(twice.g[0])
+    optim.adamw_step(s.p, [twice.g[0], twice.g[0]], s.m, s.v, s.steps, **HYPER)
+    again = Set([300, 300])
+    optim.adamw_step(again.p, twice.g, again.m, again.v, again.steps, **HYPER)
+    for x, y in zip(s.p + s.m + s.v, again.p + again.m + again.v):
+        assert torch.equal(x, y)
+
+
 def test_square_sums():
     g = torch.Generator().manual_seed(0)
     xs = [torch.randn(n, generator=g).to(t).cuda() for n, t in ((0, F32), (1, F16), (70001, F32), (4097, BF16), (9, F32))]

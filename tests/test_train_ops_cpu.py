@@ -175,6 +175,31 @@ def test_state_dict_of_8_bit_moments_survives_loading_into_a_16_bit_model():
         assert b.state[q][name].data_ptr() != value.data_ptr()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_state_dict_of_torchs_adam_is_taken_over_in_the_weights_layout(dtype):
+    def make():
+        torch.manual_seed(0)
+        return [torch.nn.Parameter(torch.randn(4, 6, 3, 3).to(dtype)), torch.nn.Parameter(torch.randn(()).to(dtype))]
+    params = make()
+    a = torch.optim.Adam(params, lr=0.5, betas=(0.5, 0.75))
+    for p in params:
+        p.grad = torch.randn_like(p)
+    a.step()
+    saved = a.state_dict()
+    saved["state"][1]["step"] = 1                               # as old files have it
+    mine = make()
+    mine[0].data = mine[0].data.to(memory_format=torch.channels_last)
+    b = optim.AdamW(mine, lr=torch.tensor(0.1))
+    b.load_state_dict(saved)
+    assert b.param_groups[0]["lr"] == 0.5 and b.param_groups[0]["betas"] == (0.5, 0.75)
+    for p, q in zip(params, mine):
+        state = b.state[q]
+        assert state["step"].dtype == torch.float32 and state["step"].numel() == 1 and state["step"] == 1
+        for name in ("exp_avg", "exp_avg_sq"):
+            assert state[name].dtype == torch.float32 and state[name].stride() == q.stride() and not state[name].requires_grad
+            assert torch.equal(state[name], a.state[p][name].float())
+
+
 def test_optimizer_can_be_copied_and_pickled():
     import copy
     import pickle
