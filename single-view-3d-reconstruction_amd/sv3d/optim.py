@@ -140,8 +140,20 @@ class AdamW(torch.optim.Optimizer):
         """As every optimizer's, also from `torch.optim.Adam`'s and `AdamW`'s.  8-bit codes stay what they are, moments of
         any other type become float32 in their weight's strides, whatever the weight's type; step counts and a
         learning rate that is a tensor go to the weights' device."""
+        found = {}
+        # Hooks that the caller registered before loading may change or replace the dict, those after it the state: the dict
+        # is looked at behind the former, what it holds is converted ahead of the latter.
+        hooks = (self.register_load_state_dict_pre_hook(lambda _, d: found.update(d)),
+                 self.register_load_state_dict_post_hook(lambda _: self._take_over(found), prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _take_over(self, state_dict):
+        """The dict's state in place of what the base class made of it, which is of the weights' types."""
         kept = state_dict["state"]
-        super().load_state_dict(state_dict)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, params):

@@ -1,0 +1,100 @@
+"""State dicts of the fused optimizer, without a GPU: hooks around loading, and checkpoints whose options the step does
+not have."""
+import copy
+
+import pytest
+import torch
+
+from sv3d import optim
+
+
+def stepped(cls=torch.optim.Adam, sizes=(3, 3), **kw):
+    """A state dict of torch's optimizer after one step."""
+    g = torch.Generator().manual_seed(0)
+    params = [torch.nn.Parameter(torch.randn(n, generator=g)) for n in sizes]
+    a = cls(params, **kw)
+    for p in params:
+        p.grad = torch.randn(p.shape, generator=g)
+    a.step()
+    return a.state_dict()
+
+
+def fresh(sizes=(3, 3), **kw):
+    params = [torch.nn.Parameter(torch.zeros(n)) for n in sizes]
+    return params, optim.AdamW(params, **kw)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_what_a_hook_before_loading_makes_of_the_state_is_loaded(in_place):
+    saved = stepped()
+
+    def sevens(_, d):
+        if not in_place:
+            d = copy.deepcopy(d)
+        for state in d["state"].values():
+            state["exp_avg"] = torch.full_like(state["exp_avg"], 7.0)
+        return None if in_place else d
+
+    params, b = fresh()
+    b.register_load_state_dict_pre_hook(sevens)
+    b.load_state_dict(copy.deepcopy(saved))
+    for i, p in enumerate(params):
+        assert bool((b.state[p]["exp_avg"] == 7.0).all())
+        assert torch.equal(b.state[p]["exp_avg_sq"], saved["state"][i]["exp_avg_sq"])
+
+
+def test_a_hook_that_reorders_the_parameters_gives_each_its_own_moments():
+    saved = stepped()
+
+    def swapped(_, d):
+        return {"state": {0: d["state"][1], 1: d["state"][0]}, "param_groups": d["param_groups"]}
+
+    params, b = fresh()
+    b.register_load_state_dict_pre_hook(swapped)
+    b.load_state_dict(saved)
+    for p, i in zip(params, (1, 0)):
+        for name in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(b.state[p][name], saved["state"][i][name])
+
+
+def test_a_hook_that_drops_state_or_sets_options_before_loading():
+    saved = stepped(lr=0.5)
+
+    def fewer(_, d):
+        d = copy.deepcopy(d)
+        del d["state"][1]
+        d["param_groups"][0]["lr"] = torch.tensor(0.25, dtype=torch.float64)
+        return d
+
+    params, b = fresh()
+    b.register_load_state_dict_pre_hook(fewer)
+    b.load_state_dict(saved)
+    assert torch.equal(b.state[params[0]]["exp_avg"], saved["state"][0]["exp_avg"]) and not b.state.get(params[1])
+    lr = b.param_groups[0]["lr"]
+    assert lr.dtype == torch.float32 and lr == 0.25
+
+
+def test_a_hook_after_loading_has_the_last_word():
+    params, b = fresh()
+
+    def zeros(o):
+        assert all(s["exp_avg"].dtype == torch.float32 for s in o.state.values())
+        for s in o.state.values():
+            s["exp_avg"] = torch.zeros_like(s["exp_avg"])
+
+    b.register_load_state_dict_post_hook(zeros)
+    b.load_state_dict(stepped())
+    assert all(not b.state[p]["exp_avg"].any() and b.state[p]["exp_avg_sq"].any() for p in params)
+
+
+def test_loading_leaves_no_hooks_behind():
+    params, b = fresh()
+    saved = stepped()
+    b.load_state_dict(saved)
+    with pytest.raises(ValueError):
+        b.load_state_dict(stepped(sizes=(3, 3, 3)))
+    c = copy.deepcopy(saved)
+    c["state"][0]["exp_avg"] += 1
+    b.load_state_dict(c)
+    assert torch.equal(b.state[params[0]]["exp_avg"], c["state"][0]["exp_avg"])
+    assert not b._optimizer_load_state_dict_pre_hooks and not b._optimizer_load_state_dict_post_hooks
