@@ -139,11 +139,22 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """As every optimizer's, also from `torch.optim.Adam`'s and `AdamW`'s.  8-bit codes stay what they are, moments of
         any other type become float32 in their weight's strides, whatever the weight's type; step counts and a
-        learning rate that is a tensor go to the weights' device."""
+        learning rate that is a tensor go to the weights' device.  A dict of another update is refused: one with
+        `amsgrad`, or of an `Adam` whose `weight_decay` is part of the gradient."""
         found = {}
+
+        def take(_, d):
+            for group in d["param_groups"]:
+                if group.get("amsgrad"):
+                    raise ValueError("the saved optimizer has amsgrad=True, which this AdamW does not have")
+                if group.get("weight_decay", 0) != 0 and not group.get("decoupled_weight_decay", True):
+                    raise ValueError("the saved optimizer adds weight_decay=%r to the gradients (Adam), this AdamW takes it off "
+                                     "the weights" % (group["weight_decay"],))
+            found.update(d)
+
         # Hooks that the caller registered before loading may change or replace the dict, those after it the state: the dict
         # is looked at behind the former, what it holds is converted ahead of the latter.
-        hooks = (self.register_load_state_dict_pre_hook(lambda _, d: found.update(d)),
+        hooks = (self.register_load_state_dict_pre_hook(take),
                  self.register_load_state_dict_post_hook(lambda _: self._take_over(found), prepend=True))
         try:
             super().load_state_dict(state_dict)

@@ -98,3 +98,31 @@ def test_loading_leaves_no_hooks_behind():
     b.load_state_dict(c)
     assert torch.equal(b.state[params[0]]["exp_avg"], c["state"][0]["exp_avg"])
     assert not b._optimizer_load_state_dict_pre_hooks and not b._optimizer_load_state_dict_post_hooks
+
+
+@pytest.mark.parametrize("cls, kw, words", [
+    (torch.optim.Adam, dict(amsgrad=True), "amsgrad"),
+    (torch.optim.AdamW, dict(amsgrad=True), "amsgrad"),
+    (torch.optim.Adam, dict(weight_decay=0.1), "weight_decay"),         # added to the gradient, not taken off the weight
+])
+def test_a_checkpoint_whose_update_is_another_one_is_refused(cls, kw, words):
+    params, b = fresh(lr=0.125)
+    b.load_state_dict(stepped())
+    before = copy.deepcopy(b.state_dict())
+    with pytest.raises(ValueError, match=words):
+        b.load_state_dict(stepped(cls, **kw))
+    after = b.state_dict()
+    assert after["param_groups"] == before["param_groups"]
+    for i in (0, 1):
+        assert all(torch.equal(after["state"][i][k], v) for k, v in before["state"][i].items())
+
+
+def test_a_checkpoint_of_the_same_update_is_taken():
+    for cls, kw in ((torch.optim.Adam, {}), (torch.optim.AdamW, dict(weight_decay=0.1)), (torch.optim.AdamW, dict(maximize=True)),
+                    (torch.optim.Adam, dict(foreach=True))):
+        saved = stepped(cls, **kw)
+        params, b = fresh()
+        b.load_state_dict(saved)
+        assert torch.equal(b.state[params[1]]["exp_avg"], saved["state"][1]["exp_avg"])
+        for name in ("weight_decay", "maximize"):
+            assert b.param_groups[0][name] == saved["param_groups"][0][name]
