@@ -177,5 +177,7 @@ class AdamW(torch.optim.Optimizer):
                     value = value.detach().to(device=p.device, copy=True)
                 self.state[p][name] = value
         for group in self.param_groups:
+            for name, value in self.defaults.items():       # what older versions of torch did not save
+                group.setdefault(name, value)
             if torch.is_tensor(group["lr"]) and group["params"]:
                 group["lr"] = group["lr"].detach().to(device=group["params"][0].device, dtype=torch.float32, copy=True)

@@ -126,3 +126,18 @@ def test_a_checkpoint_of_the_same_update_is_taken():
         assert torch.equal(b.state[params[1]]["exp_avg"], saved["state"][1]["exp_avg"])
         for name in ("weight_decay", "maximize"):
             assert b.param_groups[0][name] == saved["param_groups"][0][name]
+
+
+def test_options_that_an_old_checkpoint_lacks_are_the_constructors():
+    saved = stepped()
+    for name in ("maximize", "amsgrad", "decoupled_weight_decay"):
+        del saved["param_groups"][0][name]
+    params, b = fresh(maximize=True)
+    b.load_state_dict(saved)
+    assert b.param_groups[0]["maximize"] is True
+    p = torch.nn.Parameter(torch.zeros(3, device="meta"))
+    c = optim.AdamW([p])
+    del saved["param_groups"][0]["params"][1], saved["state"][1]
+    c.load_state_dict(saved)
+    p.grad = torch.zeros_like(p)
+    c.step()
