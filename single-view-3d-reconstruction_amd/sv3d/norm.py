@@ -3,6 +3,8 @@
 The transformer camera head of the reference's network (nnutils/mesh_net.py:468-536) is made of blocks that each
 end in one.  GPU tensors only.
 """
+import math
+
 import torch
 
 from .ops import call
@@ -25,10 +27,20 @@ class LayerNorm(torch.nn.LayerNorm):
         return layer_norm(x, self.normalized_shape, self.weight, self.bias, self.eps)
 
 
+_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _computable(m):
+    """Whether the kernel has the layer's type and size (a layer without weights takes the type of what it is given)."""
+    size = math.prod(m.normalized_shape)
+    return 0 < size <= 1 << 24 and all(p is None or p.dtype in _TYPES for p in (m.weight, m.bias))
+
+
 def convert_layer_norm(module):
     """Turns every `torch.nn.LayerNorm` inside `module` (or `module` itself) into this `LayerNorm`, in place:
-    parameters, hooks and state dict stay.  Subclasses are left alone.  Returns the number of layers changed."""
-    found = [m for m in module.modules() if type(m) is torch.nn.LayerNorm]
+    parameters, hooks and state dict stay.  Subclasses are left alone, and so are layers that the kernel does not compute:
+    with float64 weights, or over none or more than 2^24 elements.  Returns the number of layers changed."""
+    found = [m for m in module.modules() if type(m) is torch.nn.LayerNorm and _computable(m)]
     for m in found:
         m.__class__ = LayerNorm
     return len(found)

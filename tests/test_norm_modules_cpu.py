@@ -1,0 +1,21 @@
+"""Layer norm as a module and in the graph, without a GPU: which modules are converted, what the graph's node keeps, what
+it says where it has no derivative."""
+import pytest
+import torch
+
+import sv3d
+from sv3d import norm
+
+
+def test_conversion_leaves_layers_alone_that_the_kernel_does_not_compute():
+    N = torch.nn.LayerNorm
+    half_double = N(4)
+    half_double.bias = torch.nn.Parameter(torch.zeros(4, dtype=torch.float64))
+    m = torch.nn.ModuleList([N(4), N(4, dtype=torch.float64), N(4, bias=False, dtype=torch.float64), half_double,
+                             N(4, elementwise_affine=False), N(4, dtype=torch.bfloat16), N(4).half(), N((0, 4)),
+                             N((1 << 24) + 1, elementwise_affine=False)])
+    assert sv3d.convert_layer_norm(m) == 4
+    assert [type(x) is norm.LayerNorm for x in m] == [True, False, False, False, True, True, True, False, False]
+    x = torch.randn(3, 4, dtype=torch.float64)
+    for k in (1, 2):
+        assert m[k](x).dtype == torch.float64
