@@ -217,8 +217,7 @@ NormOut layer_norm_backward_meta(const Tensor &dy, const Tensor &x, IntList shap
 // 6 to 12 us more per backward, of the 65 us that forward and backward of a small layer take on the host.
 struct LayerNormBackward : public torch::autograd::Node {
     using torch::autograd::Node::Node;
-    torch::autograd::SavedVariable x, weight, bias;
-    Tensor mean, rstd;
+    torch::autograd::SavedVariable x, weight, bias, mean, rstd;
     std::vector<int64_t> shape;
     bool released = false;
 
@@ -230,8 +229,8 @@ struct LayerNormBackward : public torch::autograd::Node {
         x.reset_data();
         weight.reset_data();
         bias.reset_data();
-        mean.reset();
-        rstd.reset();
+        mean.reset_data();
+        rstd.reset_data();
         released = true;
     }
 
@@ -250,7 +249,7 @@ struct LayerNormBackward : public torch::autograd::Node {
         static auto op = find_op<NormOut(const Tensor &, const Tensor &, IntList, const optional<Tensor> &,
                                          const optional<Tensor> &, const Tensor &, const Tensor &, bool, bool, bool)>(
             "sv3d::layer_norm_backward");
-        const auto g = op.call(grads[0], xt, shape, wt, bt, mean, rstd, need[0], need[1], need[2]);
+        const auto g = op.call(grads[0], xt, shape, wt, bt, mean.unpack(), rstd.unpack(), need[0], need[1], need[2]);
         if (need[0]) out[0] = std::get<0>(g);
         if (need[1]) out[1] = std::get<1>(g);
         if (need[2]) out[2] = std::get<2>(g);
@@ -273,16 +272,18 @@ Tensor layer_norm_autograd(const Tensor &x, IntList shape, const optional<Tensor
     }
     auto node = std::shared_ptr<LayerNormBackward>(new LayerNormBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(x, w, b));
-    Tensor y;
+    Tensor y, mean, rstd;
     {
         at::AutoDispatchBelowADInplaceOrView guard;
         static auto op = find_op<NormOut(const Tensor &, IntList, const optional<Tensor> &, const optional<Tensor> &, double,
                                          bool)>("sv3d::layer_norm_stats");
-        std::tie(y, node->mean, node->rstd) = op.call(x, shape, weight, bias, eps, f32_out);
+        std::tie(y, mean, rstd) = op.call(x, shape, weight, bias, eps, f32_out);
     }
     node->x = torch::autograd::SavedVariable(x, false);
     node->weight = torch::autograd::SavedVariable(w, false);
     node->bias = torch::autograd::SavedVariable(b, false);
+    node->mean = torch::autograd::SavedVariable(mean, false);
+    node->rstd = torch::autograd::SavedVariable(rstd, false);
     node->shape = shape.vec();
     torch::autograd::set_history(y, node);
     return y;

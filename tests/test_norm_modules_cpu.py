@@ -19,3 +19,27 @@ def test_conversion_leaves_layers_alone_that_the_kernel_does_not_compute():
     x = torch.randn(3, 4, dtype=torch.float64)
     for k in (1, 2):
         assert m[k](x).dtype == torch.float64
+
+
+def meta(*shape):
+    return torch.empty(shape, device="meta")
+
+
+def test_hooks_on_saved_tensors_see_all_that_the_graph_keeps():
+    """x, weight, bias and both statistics of the rows; what the hooks hand back is what the backward takes."""
+    packed, unpacked = [], []
+
+    def pack(t):
+        packed.append(t)
+        return t
+
+    def unpack(t):
+        unpacked.append(t)
+        return t
+
+    x, w, b = (t.requires_grad_() for t in (meta(6, 8), meta(8), meta(8)))
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        y = norm.layer_norm(x, 8, w, b)
+    assert [tuple(t.shape) for t in packed] == [(6, 8), (8,), (8,), (6,), (6,)]
+    assert [t.shape for t in torch.autograd.grad(y, (x, w, b), meta(6, 8))] == [x.shape, w.shape, b.shape]
+    assert len(unpacked) == len(packed)
