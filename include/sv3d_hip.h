@@ -395,7 +395,7 @@ int sv3d_grad_square_sums(const sv3d_adamw_tensor *tensors, int32_t num_tensors,
  *   g  = grad / S * min(1, max_norm / (G + 1e-6))       (no factor if max_norm is 0)
  *   t  = step + 1;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   param = param (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
- * in fp32 (an eps below 2^-63 counts as 2^-63); the weight is rounded to its type to nearest, 8-bit
+ * in fp32 (where v is 0, an eps below 2^-63 counts as 2^-63); the weight is rounded to its type to nearest, 8-bit
  * moments are rounded up or down with the probability of what is cut off, decided by a hash of
  * (element, t, seed), and a positive exp_avg_sq never becomes zero.  `maximize` negates g.  If *found_inf is
  * not 0 nothing is changed.  lr is read from `lr_device` where that is not NULL.  With max_norm > 0

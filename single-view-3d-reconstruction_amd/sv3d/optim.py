@@ -27,6 +27,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, scales=None, lr=1
     block of 128, rounded up or down with the probability of what is cut off, by a hash of element, step and `seed`
     (see `moment_values`).  `steps` are one-element float32 tensors on the device.
 
+    Where the second moment is zero an `eps` below 2^-63 counts as 2^-63: a weight that never had a gradient stays.
+
     `lr` may be a one-element float32 tensor on the device; `grad_scale` and `found_inf` are such tensors or None, and
     with a `found_inf` that is not 0 nothing changes.  `square_sums` (of `grad_square_sums`) says whose norm is meant
     where that is not the norm of `grads` alone."""

@@ -1,0 +1,87 @@
+"""What the optimizer step rounds, and where: the root and the quotient of the update, second moments below float32's normal
+numbers."""
+import pytest
+import torch
+
+from oracle import train_oracle as to
+from sv3d import optim
+from test_adamw_gpu import BF16, F16
+
+pytestmark = pytest.mark.gpu
+
+
+def one(values, bits=32, step=0.0):
+    """Lists of one tensor: zero weights with the gradients `values` and no moments yet."""
+    g = values.cuda()
+    p = torch.zeros_like(g)
+    if bits == 32:
+        m, v, e = torch.zeros_like(g), torch.zeros_like(g), None
+    else:
+        m, v = (torch.zeros(g.shape, dtype=torch.uint8, device="cuda") for _ in range(2))
+        e = [torch.zeros(-(-g.numel() // 128), 2, dtype=torch.uint8, device="cuda")]
+    return p, g, m, v, torch.tensor(step).cuda(), e
+
+
+def run(p, g, m, v, s, e, **kw):
+    optim.adamw_step([p], [g], [m], [v], [s], scales=e, **{"weight_decay": 0.0, **kw})
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [3000, 100000])         # in one workgroup, and in many
+def test_root_and_quotient_are_rounded_to_nearest(bits, n):
+    """Without memory (both betas 0) the step of a gradient g is g / sqrt(g^2).  The root of a rounded square is |g| again
+    (no overflow, no underflow) and a number divided by itself is 1: the step is lr exactly, whatever g is."""
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, generator=g) * 10.0 ** (3 * torch.randn(n, generator=g))
+    t = one(x, bits)
+    run(*t, lr=0.5, betas=(0.0, 0.0), eps=0.0)
+    assert torch.equal(t[0].cpu(), -0.5 * x.sign())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [3000, 100000])
+@pytest.mark.parametrize("eps", [0.0, 1e-22])
+def test_first_steps_of_gradients_whose_squares_are_not_normal(bits, n, eps):
+    """g from 1e-19 to 1e-17 at the first step: v = 1e-3 g^2 lies below 2^-126 in steps of 2^-149, half a step of which is
+    up to 2^-150 / 1e-41 of it, 7e-5, and half as much of the root.  A tenth of g's size is far outside."""
+    g = torch.Generator().manual_seed(n)
+    x = 10.0 ** (-19 + 2 * torch.rand(n, generator=g)) * (torch.randint(0, 2, (n,), generator=g) * 2 - 1)
+    p, gr, m, v, s, e = one(x, bits)
+    run(p, gr, m, v, s, e, lr=1.0, eps=eps)
+    w = x.double()
+    want = to.adamw(torch.zeros(n, dtype=torch.float64), w, 0 * w, 0 * w, 0.0, lr=1.0, betas=(0.9, 0.999), eps=eps, weight_decay=0.0)
+    v1 = 1e-3 * w * w
+    # the product (1 - beta2) g and the square are each rounded; 4 covers the double rounding of both near the border
+    room = 4 * 2.0 ** -150 / v1 + 16 * 2.0 ** -24
+    assert bool(((p.cpu().double() - want["p"]).abs() <= room).all()), float(((p.cpu().double() - want["p"]).abs() / room).max())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [3000, 100000])
+@pytest.mark.parametrize("t", [F16, BF16])
+def test_the_same_for_16_bit_weights(bits, n, t):
+    """The root's and the quotient's errors, a few 2^-23, are far below half a step of the weight: the step without memory is lr
+    again, and first steps of gradients whose squares are not normal are +-1 (bf16, whose numbers go that far down; what the
+    squares lose, 3e-4 at most, is below half a step as well)."""
+    g = torch.Generator().manual_seed(n)
+    x = (torch.randn(n, generator=g) * 10.0 ** torch.randn(n, generator=g)).to(t)
+    x[x == 0] = 1.0
+    a = one(x, bits)
+    a = (*a[:2], *(s if s.dtype == torch.uint8 else s.float() for s in a[2:4]), *a[4:])
+    run(*a, lr=0.5, betas=(0.0, 0.0), eps=0.0)
+    assert torch.equal(a[0].cpu(), (-0.5 * x.sign()).to(t))
+    if t is BF16:
+        x = (10.0 ** (-19 + 2 * torch.rand(n, generator=g)) * x.sign().float()).to(t)
+        a = one(x, bits)
+        a = (*a[:2], *(s if s.dtype == torch.uint8 else s.float() for s in a[2:4]), *a[4:])
+        run(*a, lr=1.0, eps=0.0)
+        assert torch.equal(a[0].cpu(), -x.sign())
+
+
+@pytest.mark.parametrize("n", [300, 40000])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_weights_that_never_had_a_gradient_stay_without_eps(bits, n):
+    t = one(torch.zeros(n), bits)
+    t[0].fill_(0.25)
+    run(*t, lr=1.0, eps=0.0)
+    assert bool((t[0] == 0.25).all())
