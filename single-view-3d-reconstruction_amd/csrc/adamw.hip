@@ -5,6 +5,7 @@
 // be kept up to date), at most kTable of them per launch, cut into chunks; a workgroup looks up its chunk's tensor.
 #include "element.h"
 
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -84,12 +85,13 @@ __global__ __launch_bounds__(kThreads) void grad_square_sums_kernel(SumTable t, 
 // ---- what each tensor's update multiplies by -------------------------------------------------------
 struct Factors {
     float grad;         // unscaling, clipping and sign
-    float decay;        // 1 - lr weight_decay
     float rate;         // lr / (1 - beta1^t)
     float root;         // 1 / sqrt(1 - beta2^t)
+    float small_root;   // 2^-16 of that
+    float decay;        // lr weight_decay
+    float keep;         // 1 - lr weight_decay
     uint32_t key;       // of the dither
     int32_t skip;
-    int32_t pad[2];
 };
 
 // What the kernels need of the call's parameters.
@@ -125,12 +127,13 @@ __device__ inline Factors factors_of(const Scalars &p, float *step)
     if (!skip) *step = n;
     Factors f;
     f.grad = 0.f;
-    f.decay = (float)(1.0 - lr * p.weight_decay);
     f.rate = (float)(lr / -expm1((double)n * p.log_b1));
     f.root = (float)(1.0 / sqrt(-expm1((double)n * p.log_b2)));
+    f.small_root = f.root * 0x1p-16f;
+    f.decay = (float)(lr * p.weight_decay);
+    f.keep = (float)(1.0 - lr * p.weight_decay);
     f.key = (uint32_t)n * 0x9E3779B1u + p.seed * 0x6A09E667u;
     f.skip = skip;
-    f.pad[0] = f.pad[1] = 0;
     return f;
 }
 
@@ -279,10 +282,13 @@ static_assert(sizeof(Table) + sizeof(Betas) + 16 <= 4096, "kernel arguments");
 
 // New moments and weight.  For fp32 weights the root and the quotient are rounded to nearest.  For 16-bit weights they are
 // the hardware's, off by one unit in fp32's last place where the exact ones are off by half: the weight that the step
-// goes into is rounded to 8 or 11 of its 24 bits.  (134 M bf16 weights with 8-bit moments 353 us, 399 with the exact ones; 62 M
-// fp32 weights wait for memory: 305.9 with the exact ones and 305.4 with the hardware's, 268.5 and 267.5 with 8-bit moments.)
+// goes into is rounded to 8 or 11 of its 24 bits.  (134 M bf16 weights with 8-bit moments 357 us, 399 with the exact ones; 62 M
+// fp32 weights wait for memory: 305 with either, with 8-bit moments 269 with the exact ones and 268 with the hardware's.)
 // The hardware's root takes numbers below the normal ones (2^-126) for zero, and squares of first gradients get there:
 // small ones are scaled by 2^32.
+// The decay of an fp32 weight is added to the step and both are taken off with one rounding: a factor 1 - decay would be
+// 2^-24 off, more than a decay of 1e-8 and a fifth of one of 1e-7, the same way in every step.  A weight that is an infinity
+// stays one.  The rounding of a 16-bit weight is far above that.
 // A second moment of zero, that of an element without a gradient or of squares that fp32 does not hold, has at least
 // 2^-63 (the root of the smallest normal number) in place of eps: there the quotient is 0/0 or nearly so.
 template <class T>
@@ -292,15 +298,15 @@ __device__ inline float step_of(float p, float &m, float &v, float g, const Beta
     m = fmaf(b.c1, g, b.b1 * m);
     v = fmaf(b.c2 * g, g, b.b2 * v);
     const float eps = v > 0.f ? b.eps : b.eps_of_zero;
-    float u;
     if constexpr (sizeof(T) == 4) {
-        u = m / fmaf(sqrtf(v), f.root, eps);
+        const float u = m / fmaf(sqrtf(v), f.root, eps);
+        return p - fmaf(f.rate, u, f.decay * __builtin_amdgcn_fmed3f(p, -FLT_MAX, FLT_MAX));
     } else {
         const bool small = v < 0x1p-96f;
         const float root = __builtin_amdgcn_sqrtf(v * (small ? 0x1p32f : 1.f));
-        u = m * __builtin_amdgcn_rcpf(fmaf(root, small ? f.root * 0x1p-16f : f.root, eps));
+        const float u = m * __builtin_amdgcn_rcpf(fmaf(root, small ? f.small_root : f.root, eps));
+        return fmaf(-f.rate, u, p * f.keep);
     }
-    return fmaf(-f.rate, u, p * f.decay);
 }
 
 // The tensor of chunk `chunk`: the lanes look at the table's entries at once, two each.

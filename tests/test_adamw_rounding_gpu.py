@@ -1,5 +1,7 @@
 """What the optimizer step rounds, and where: the root and the quotient of the update, second moments below float32's normal
-numbers."""
+numbers, decays far below a weight's last bit."""
+import math
+
 import pytest
 import torch
 
@@ -85,3 +87,51 @@ def test_weights_that_never_had_a_gradient_stay_without_eps(bits, n):
     t[0].fill_(0.25)
     run(*t, lr=1.0, eps=0.0)
     assert bool((t[0] == 0.25).all())
+
+
+@pytest.mark.parametrize("n, bits", [(65536, 32), (65536, 8), (8192, 32)])
+@pytest.mark.parametrize("lr, weight_decay", [(1e-5, 0.01), (2e-6, 0.01), (1e-4, 0.01)])
+def test_small_decays_add_up(n, bits, lr, weight_decay):
+    """Decays of 1e-7, 2e-8 and 1e-6 of weights in [0.5, 1), whose last bit is 2^-24: each step rounds a weight by half of
+    that at most, at random (the update's size, 1e-5 of many digits, decides), so the mean over n weights of what
+    T steps add up to is off by 2^-24 / sqrt(12) * sqrt(T / n) or so.  8 of those, and the decay's own size by 1e-3.
+    The first step is not at random: without a memory of others every update is lr or -lr.  With lr = 33.55 last bits and a
+    decay of 0.17 to 0.33 of one, 33.72 to 33.88 become 34 and -33.38 to -33.22 become -33, 0.25 too much on average of both
+    for all weights at once: up to half a last bit, 2^-25, for an lr in general."""
+    steps = 200
+    g = torch.Generator().manual_seed(5)
+    start = 0.5 + 0.5 * torch.rand(n, generator=g)
+    start = start.clamp(0.51, 0.99)
+    p, gr, m, v, s, e = one(torch.zeros(n), bits)
+    q, gq, mq, vq, sq, eq = one(torch.zeros(n), bits)
+    p.copy_(start)
+    q.copy_(start)
+    moved = torch.zeros(n, dtype=torch.float64, device="cuda")       # what the updates without decay add up to
+    for _ in range(steps):
+        x = torch.randn(n, generator=g).cuda()
+        gr.copy_(x)
+        gq.copy_(x)
+        run(p, gr, m, v, s, e, lr=lr, weight_decay=weight_decay, seed=3)
+        q.zero_()
+        run(q, gq, mq, vq, sq, eq, lr=lr, seed=3)
+        moved += q.double()
+    got = float((start.double() - p.cpu().double() + moved.cpu()).mean())
+    # the sum over the steps of lr wd p, with p as it was: it moves by 200 lr at most
+    want = steps * lr * weight_decay * float(start.double().mean())
+    room = 2.0 ** -25 + 8 * 2.0 ** -24 / math.sqrt(12) * math.sqrt(steps / n) + want * (1e-3 + steps * lr)
+    assert abs(got - want) <= room, (got, want, room)
+
+
+@pytest.mark.parametrize("weight_decay", [0.0, 0.1])
+@pytest.mark.parametrize("n", [300, 40000])
+def test_infinite_weights_stay_what_they_are(weight_decay, n):
+    """As a mask that is held as a weight: an infinity less its decay is that infinity."""
+    p, g, m, v, s, e = one(torch.zeros(n))
+    p[::3], p[1::3] = math.inf, -math.inf
+    want = p.clone()
+    run(p, g, m, v, s, e, lr=0.01, weight_decay=weight_decay)
+    assert torch.equal(p, want)
+    half = want.to(BF16)
+    gh = torch.zeros_like(half)
+    run(half, gh, m, v, s, e, lr=0.01, weight_decay=weight_decay)
+    assert torch.equal(half, want.to(BF16))
