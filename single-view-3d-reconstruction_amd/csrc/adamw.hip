@@ -324,8 +324,8 @@ __device__ inline int tensor_of(const int32_t *first, int count, int chunk)
 // chunk does.  Weights and moments are read and written past the caches: nothing of this step reads them again, and what
 // the step before left to be written back does not come in between (62 M weights, 32-bit moments, clipped: 383 us through
 // the caches, 303 us past them; only the loads or only the stores gain nothing).  Gradients are read past the caches if no
-// norm was taken of them just before (134 M bf16 gradients: 367 and 353 us), out of the caches if one was (62 M: 303 and
-// 291 us with 8-bit moments).
+// norm was taken of them just before (134 M bf16 gradients: 367 and 353 us), out of the caches if one was, by this call or by
+// the caller for several of them (62 M with 8-bit moments: 303 and 291 us; in two groups 221 and 206).
 template <bool WHOLE, class T, int V, bool STREAM = true>
 __device__ inline Words<T, V> load_some(const T *p, int n)
 {
@@ -750,10 +750,10 @@ extern "C" int sv3d_adamw_step(const sv3d_adamw_params *p, const sv3d_adamw_tens
                      (float)p->eps, (float)(p->eps > 0x1p-63 ? p->eps : 0x1p-63)};
     if (small_call(p, tensors, num_tensors)) return small_step(scalars, b, tensors, num_tensors, (hipStream_t)stream);
     Factors *factors = (Factors *)workspace;
-    const bool clip = p->max_norm > 0.0, read_before = clip && !p->square_sums;
+    const bool clip = p->max_norm > 0.0;
     const double *sums = p->square_sums;
     int32_t num_sums = clip ? p->num_square_sums : 0;
-    if (read_before) {
+    if (clip && !p->square_sums) {
         num_sums = (int32_t)((need - num_tensors * sizeof(Factors)) / sizeof(double));
         double *own = (double *)(factors + num_tensors);
         if (const int st = sv3d_grad_square_sums(tensors, num_tensors, own, num_sums, stream)) return st;
@@ -787,8 +787,8 @@ extern "C" int sv3d_adamw_step(const sv3d_adamw_params *p, const sv3d_adamw_tens
                         t.odd[k] = (uint8_t)(from >> 31 & 1);
                     }
                     for (int k = 0; k <= n; ++k) t.first[k] = first[k];
-                    const auto kernel = bits == 32 ? (read_before ? adamw_kernel<E, false> : adamw_kernel<E, true>)
-                                                   : (read_before ? adamw8_kernel<E, false> : adamw8_kernel<E, true>);
+                    const auto kernel = bits == 32 ? (clip ? adamw_kernel<E, false> : adamw_kernel<E, true>)
+                                                   : (clip ? adamw8_kernel<E, false> : adamw8_kernel<E, true>);
                     hipLaunchKernelGGL(kernel, dim3(first[n]), dim3(kThreads), 0, (hipStream_t)stream, t, b, factors);
                     return launch_status();
                 });
