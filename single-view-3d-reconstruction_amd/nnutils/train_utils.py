@@ -418,6 +418,12 @@ class Trainer(object):
                     self._zero_grads()
                     self._forward_backward(total_steps, scaler)
             torch.cuda.current_stream(self.device).wait_stream(side)
+            if whole:
+                # weights that got their first gradient in these passes have no optimizer state yet, and what a
+                # capture makes is made anew by every replay
+                for opt in [self.optimizer] + ([self.optimizer_2] if self._second_optimizer() else []):
+                    if self._fused_step(opt):
+                        opt.make_state()
             # nothing made by those passes may be released inside the capture (a tensor with autograd
             # history that was allocated on the side stream and dies during capture ends the capture
             # in a segmentation fault on this PyTorch-ROCm build): their loss goes now

@@ -60,7 +60,8 @@ class AdamW(torch.optim.Optimizer):
     unscaled gradients (a tensor on the device) where `max_norm` is set.
 
     Works with `torch.amp.GradScaler` (call `scaler.step(optimizer)` alone: unscaling happens inside) and inside a HIP
-    graph once the first step has made the state; a learning rate that changes under a captured step is a tensor."""
+    graph once the first step or `make_state` has made the state; a learning rate that changes under a captured step is a
+    tensor."""
 
     _step_supports_amp_scaling = True       # GradScaler hands over grad_scale and found_inf instead of unscaling
 
@@ -89,7 +90,8 @@ class AdamW(torch.optim.Optimizer):
 
     def _new_state(self, p):
         if p.is_cuda and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("sv3d.optim.AdamW makes its state on a tensor's first step, which must come before the capture")
+            raise RuntimeError("sv3d.optim.AdamW makes a weight's state on its first step or in make_state(), one of which must come "
+                               "before the capture")
         state = {"step": torch.zeros((), dtype=torch.float32, device=p.device)}
         if self.state_bits == 8 and p.numel() >= self.min_8bit_size:
             for name in ("exp_avg", "exp_avg_sq"):
@@ -100,6 +102,15 @@ class AdamW(torch.optim.Optimizer):
             for name in ("exp_avg", "exp_avg_sq"):
                 state[name] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
         return state
+
+    @torch.no_grad()
+    def make_state(self):
+        """Makes the state of every weight that has a gradient and no state yet, as its first step would: ahead of the capture
+        of that step in a HIP graph."""
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is not None and not self.state[p]:
+                    self.state[p].update(self._new_state(p))
 
     @torch.no_grad()
     def step(self, closure=None):
