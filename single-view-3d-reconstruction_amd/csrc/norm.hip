@@ -1,7 +1,8 @@
 // Layer norm over rows of `cols` elements, forward and backward.
 //   forward:  mu = mean x, r = 1/sqrt(mean (x-mu)^2 + eps), y = (x-mu) r w + b
 //   backward: h = (x-mu) r, u = dy w, dx = r (u - mean u - h mean(u h)), dw = sum_rows dy h, db = sum_rows dy
-// Statistics, gradients and their sums are fp32; only what is stored is rounded to its type.
+// Statistics, gradients and a workgroup's sums are fp32, the join of those over the rows is double; only what is stored
+// is rounded to its type.
 #include "element.h"
 
 #include <type_traits>
@@ -429,26 +430,28 @@ __global__ __launch_bounds__(kThreads) void layer_norm_slices_kernel(
     store_pack<float, V>(out + cols, b, n);
 }
 
-// The sum over the `count` partial sums: 16 columns of one of the two gradients per workgroup, 64 threads each.
+// The sum over the `count` partial sums: 16 columns of one of the two gradients per workgroup, 64 threads each.  In
+// double: there are up to 512 of either sign, and this waits for its loads.
 template <class P>
 __global__ __launch_bounds__(1024) void layer_norm_join_kernel(const float *__restrict__ part, int count, int cols,
                                                                P *__restrict__ dweight, P *__restrict__ dbias)
 {
-    __shared__ float fold[64][17];
+    __shared__ double fold[64][17];
     P *out = blockIdx.y ? dbias : dweight;
     if (!out) return;
     const int c = blockIdx.x * 16 + threadIdx.x % 16, slice = threadIdx.x / 16;
-    float s = 0.f;
+    double s = 0.0;
     if (c < cols)
-        for (int i = slice; i < count; i += 64) s += part[(2 * (int64_t)i + blockIdx.y) * cols + c];
+        for (int i = slice; i < count; i += 64) s += (double)part[(2 * (int64_t)i + blockIdx.y) * cols + c];
     fold[slice][threadIdx.x % 16] = s;
     __syncthreads();
     if (threadIdx.x >= 256) return;
     // 16 lanes for each of the 16 columns
     const int column = threadIdx.x / 16, l = threadIdx.x % 16;
     s = (fold[l][column] + fold[l + 16][column]) + (fold[l + 32][column] + fold[l + 48][column]);
-    s = lane_sum<16>(s);
-    if (l == 0 && blockIdx.x * 16 + column < cols) out[blockIdx.x * 16 + column] = from_float<P>(s);
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) s += __shfl_xor(s, d);
+    if (l == 0 && blockIdx.x * 16 + column < cols) out[blockIdx.x * 16 + column] = from_float<P>((float)s);
 }
 
 int check(const sv3d_layer_norm_params *p)
