@@ -370,7 +370,8 @@ int sv3d_layer_norm_backward(const sv3d_layer_norm_params *p, const void *x, con
  * one of exp_avg_sq for
  *   (E ? (1 + M/8) 2^(E-15) : M/8 2^-14) * 2^(e-142),               E = c>>3, M = c & 7, 0xff NaN.
  * Bytes below 20 (exp_avg) and 34 (exp_avg_sq) count as these: all zeros is a fresh state.
- * What is written (all but grad) overlaps nothing else of a call; two tensors may have one gradient. */
+ * What is written (all but grad) overlaps nothing else of a call; two tensors may have one gradient.
+ * Addresses here and in the calls below are multiples of their element's size. */
 enum { SV3D_STATE_BLOCK = 128 };
 typedef struct sv3d_adamw_tensor {
     void *param;

@@ -585,7 +585,7 @@ int check(const sv3d_adamw_tensor *tensors, int32_t n, bool grads_only)
         if (t.numel > 0 && (!t.grad || !aligned(t.grad, type_bytes(t.type)))) return SV3D_ERR_INVALID_ARG;
         if (t.numel > ((int64_t)1 << 40)) return SV3D_ERR_UNSUPPORTED;
         if (grads_only) continue;
-        if ((t.state_bits != 8 && t.state_bits != 32) || !t.step) return SV3D_ERR_INVALID_ARG;
+        if ((t.state_bits != 8 && t.state_bits != 32) || !t.step || !aligned(t.step, 4)) return SV3D_ERR_INVALID_ARG;
         if (t.numel == 0) continue;
         if (!t.param || !t.exp_avg || !t.exp_avg_sq || !aligned(t.param, type_bytes(t.type))) return SV3D_ERR_INVALID_ARG;
         if (t.state_bits == 8 ? !t.scales : !aligned(t.exp_avg, 4) || !aligned(t.exp_avg_sq, 4)) return SV3D_ERR_INVALID_ARG;
@@ -739,6 +739,9 @@ extern "C" int sv3d_adamw_step(const sv3d_adamw_params *p, const sv3d_adamw_tens
     if (const int st = check(tensors, num_tensors, false)) return st;
     if (!(p->beta1 >= 0.0 && p->beta1 < 1.0 && p->beta2 >= 0.0 && p->beta2 < 1.0 && p->eps >= 0.0)) return SV3D_ERR_INVALID_ARG;
     if (!(p->max_norm >= 0.0) || p->num_square_sums < 0) return SV3D_ERR_INVALID_ARG;
+    if (!aligned(p->lr_device, 4) || !aligned(p->grad_scale, 4) || !aligned(p->found_inf, 4) || !aligned(p->total_norm, 4) ||
+        !aligned(p->square_sums, 8))
+        return SV3D_ERR_INVALID_ARG;
     if (num_tensors == 0) return SV3D_OK;
     size_t need = 0;
     if (const int st = sv3d_adamw_workspace(p, tensors, num_tensors, &need)) return st;
