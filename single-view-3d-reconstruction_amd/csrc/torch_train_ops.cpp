@@ -240,7 +240,8 @@ struct LayerNormBackward : public torch::autograd::Node {
         variable_list out(3);
         if (!grads[0].defined()) return out;
         TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
-        TORCH_CHECK(!at::GradMode::is_enabled(), "sv3d::layer_norm has no second derivative (create_graph=True)");
+        TORCH_CHECK(!at::GradMode::is_enabled(), "sv3d::layer_norm has no second derivative: create_graph=True asks for one, "
+                    "and so does torch.func.grad");
         const Tensor xt = x.unpack();
         optional<Tensor> wt, bt;
         if (const Tensor t = weight.unpack(); t.defined()) wt = t;

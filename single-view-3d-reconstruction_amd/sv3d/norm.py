@@ -13,9 +13,10 @@ from .ops import call
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     """`torch.nn.functional.layer_norm`: normalises over the last `len(normalized_shape)` dimensions of `x`
     (float32, float16 or bfloat16; any strides, without a copy where rows are contiguous and evenly spaced), then
-    scales and shifts by `weight` and `bias` (of x's type or float32).  Statistics, arithmetic and the sums of the
-    weights' gradients are float32; the result has x's type, under autocast float32 (as torch's).  Differentiable
-    once in x, weight and bias."""
+    scales and shifts by `weight` and `bias` (of x's type or float32).  Statistics and arithmetic are float32, and so are the
+    sums of the weights' gradients until they are joined in float64; the result has x's type, under autocast float32 (as
+    torch's).  Differentiable once in x, weight and bias, by `backward` and `torch.autograd.grad` (`create_graph=True` and
+    `torch.func.grad`, which sets it, raise)."""
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     return call("layer_norm", x, shape, weight, bias, eps, torch.is_autocast_enabled("cuda"))
 

@@ -43,3 +43,11 @@ def test_hooks_on_saved_tensors_see_all_that_the_graph_keeps():
     assert [tuple(t.shape) for t in packed] == [(6, 8), (8,), (8,), (6,), (6,)]
     assert [t.shape for t in torch.autograd.grad(y, (x, w, b), meta(6, 8))] == [x.shape, w.shape, b.shape]
     assert len(unpacked) == len(packed)
+
+
+def test_refusals_of_a_second_derivative_say_who_asks_for_one():
+    x = meta(2, 8).requires_grad_()
+    with pytest.raises(RuntimeError, match=r"second derivative.*create_graph=True.*torch\.func"):
+        torch.autograd.grad(norm.layer_norm(x, 8), x, meta(2, 8), create_graph=True)
+    with pytest.raises(RuntimeError, match=r"torch\.func"):
+        torch.func.grad(lambda t: norm.layer_norm(t, 8).sum())(meta(2, 8))
