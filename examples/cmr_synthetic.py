@@ -358,6 +358,12 @@ def parse(argv=None):
     return o
 
 
+def say(line):
+    """Prints a line in one write, so that lines of several ranks do not run into each other."""
+    sys.stdout.write(line + '\n')
+    sys.stdout.flush()
+
+
 def main(argv=None):
     o = parse(argv)
     if o.num_iter == 0:
@@ -380,12 +386,12 @@ def main(argv=None):
         Bn = o.num_hypo_cams * (2 if o.flip_pair else 1) * o.batch_size
         parts = o.num_parts if o.seg_train else 0
         renders = 1 + (parts + 7) // 8 if o.share_renders else 2 + parts
-        print('steps %d, %.1f ms/step, %.1f dataset images/s over %d rank(s) (%d rendered images x %d renders per step per rank)'
-              % (steps, 1e3 * dt / max(steps, 1), steps * o.batch_size * t.env.world_size / dt, t.env.world_size, Bn, renders))
+        say('steps %d, %.1f ms/step, %.1f dataset images/s over %d rank(s) (%d rendered images x %d renders per step per rank)'
+            % (steps, 1e3 * dt / max(steps, 1), steps * o.batch_size * t.env.world_size / dt, t.env.world_size, Bn, renders))
     if o.print_checksum:
         mods = [train_utils.unwrap(t.model), train_utils.unwrap(t.part_basis_generator)]
         total = sum(float(p.detach().double().sum()) for m in mods for p in m.parameters())
-        print('rank %d weight checksum %.12e' % (t.env.rank, total), flush=True)
+        say('rank %d weight checksum %.12e' % (t.env.rank, total))
     return t
 
 
