@@ -277,36 +277,54 @@ struct Table {
 struct Betas {
     float b1, c1, b2, c2, eps;          // c = 1 - b, taken in double
     float eps_of_zero;                  // where the second moment is zero
+    int32_t tiny_eps;                   // whether roots below 2^-63 count next to eps
 };
 static_assert(sizeof(Table) + sizeof(Betas) + 16 <= 4096, "kernel arguments");
 
 // New moments and weight.  For fp32 weights the root and the quotient are rounded to nearest.  For 16-bit weights they are
 // the hardware's, off by one unit in fp32's last place where the exact ones are off by half: the weight that the step
-// goes into is rounded to 8 or 11 of its 24 bits.  (134 M bf16 weights with 8-bit moments 357 us, 399 with the exact ones; 62 M
+// goes into is rounded to 8 or 11 of its 24 bits.  (134 M bf16 weights with 8-bit moments 354 us, 399 with the exact ones; 62 M
 // fp32 weights wait for memory: 305 with either, with 8-bit moments 269 with the exact ones and 268 with the hardware's.)
-// The hardware's root takes numbers below the normal ones (2^-126) for zero, and squares of first gradients get there:
-// small ones are scaled by 2^32.
+// The hardware's root takes numbers below the normal ones (2^-126) for zero, and squares of first gradients get there.  What
+// it leaves out of the denominator is then at most 2^-63 times the bias correction.  With an eps of 2^24 times that or more
+// (5.8e-11 for beta2 = 0.999) it is below fp32's last place; TINY, the form for a smaller eps, scales small ones by 2^32
+// (357 us in the case above: six more of some sixty instructions for each element).
 // The decay of an fp32 weight is added to the step and both are taken off with one rounding: a factor 1 - decay would be
 // 2^-24 off, more than a decay of 1e-8 and a fifth of one of 1e-7, the same way in every step.  A weight that is an infinity
 // stays one.  The rounding of a 16-bit weight is far above that.
 // A second moment of zero, that of an element without a gradient or of squares that fp32 does not hold, has at least
 // 2^-63 (the root of the smallest normal number) in place of eps: there the quotient is 0/0 or nearly so.
-template <class T>
+template <class T, bool TINY>
 __device__ inline float step_of(float p, float &m, float &v, float g, const Betas &b, const Factors &f)
 {
     g *= f.grad;
     m = fmaf(b.c1, g, b.b1 * m);
     v = fmaf(b.c2 * g, g, b.b2 * v);
-    const float eps = v > 0.f ? b.eps : b.eps_of_zero;
+    const float eps = !TINY || v > 0.f ? b.eps : b.eps_of_zero;
     if constexpr (sizeof(T) == 4) {
         const float u = m / fmaf(sqrtf(v), f.root, eps);
         return p - fmaf(f.rate, u, f.decay * __builtin_amdgcn_fmed3f(p, -FLT_MAX, FLT_MAX));
     } else {
-        const bool small = v < 0x1p-96f;
-        const float root = __builtin_amdgcn_sqrtf(v * (small ? 0x1p32f : 1.f));
+        const bool small = TINY && v < 0x1p-96f;
+        const float root = __builtin_amdgcn_sqrtf(small ? v * 0x1p32f : v);
         const float u = m * __builtin_amdgcn_rcpf(fmaf(root, small ? f.small_root : f.root, eps));
         return fmaf(-f.rate, u, p * f.keep);
     }
+}
+
+// f(a constant TINY)
+template <bool V>
+struct Bool {
+    static constexpr bool value = V;
+};
+
+template <class T, class F>
+__device__ inline void with_eps(const Betas &b, F f)
+{
+    if (sizeof(T) == 2 && !b.tiny_eps)
+        f(Bool<false>());
+    else
+        f(Bool<true>());
 }
 
 // The tensor of chunk `chunk`: the lanes look at the table's entries at once, two each.
@@ -366,12 +384,14 @@ __device__ inline void update_chunk(const Entry &e, int64_t at, int left, const 
     for (int u = 0; u < U; ++u) {
         const int o = u * kThreads * V, n = left - o;
         float np[V], nm[V], nv[V];
+        with_eps<T>(b, [&](auto tiny) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            nm[j] = wm[u][j];
-            nv[j] = wv[u][j];
-            np[j] = step_of<T>(wp[u][j], nm[j], nv[j], wg[u][j], b, f);
-        }
+            for (int j = 0; j < V; ++j) {
+                nm[j] = wm[u][j];
+                nv[j] = wv[u][j];
+                np[j] = step_of<T, decltype(tiny)::value>(wp[u][j], nm[j], nv[j], wg[u][j], b, f);
+            }
+        });
         store_some<WHOLE, float, V>(em + o, to_words<float, V>(nm), n);
         store_some<WHOLE, float, V>(ev + o, to_words<float, V>(nv), n);
         store_some<WHOLE, T, V>(p + o, to_words<T, V>(np), n);
@@ -423,9 +443,12 @@ __device__ inline void update_chunk8(const Entry &e, int64_t at, int n, uint32_t
         decode_second(bv.w[q / 4], power, v + q);
     }
     uint32_t top_m = 0, top_v = 0;
+    with_eps<T>(b, [&](auto tiny) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) np[j] = step_of<T, decltype(tiny)::value>(wp[j], m[j], v[j], wg[j], b, f);
+    });
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        np[j] = step_of<T>(wp[j], m[j], v[j], wg[j], b, f);
         top_m = max(top_m, magnitude_bits(m[j]));
         top_v = max(top_v, magnitude_bits(v[j]));
     }
@@ -750,7 +773,7 @@ extern "C" int sv3d_adamw_step(const sv3d_adamw_params *p, const sv3d_adamw_tens
     const Scalars scalars = {p->lr,         log(p->beta1), log(p->beta2), p->weight_decay, p->max_norm, p->lr_device,
                              p->grad_scale, p->found_inf,  p->total_norm, p->seed,         p->maximize};
     const Betas b = {(float)p->beta1, (float)(1.0 - p->beta1), (float)p->beta2, (float)(1.0 - p->beta2),
-                     (float)p->eps, (float)(p->eps > 0x1p-63 ? p->eps : 0x1p-63)};
+                     (float)p->eps, (float)(p->eps > 0x1p-63 ? p->eps : 0x1p-63), p->eps < 0x1p-39 / sqrt(1.0 - p->beta2)};
     if (small_call(p, tensors, num_tensors)) return small_step(scalars, b, tensors, num_tensors, (hipStream_t)stream);
     Factors *factors = (Factors *)workspace;
     const bool clip = p->max_norm > 0.0;

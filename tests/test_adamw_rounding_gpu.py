@@ -80,6 +80,23 @@ def test_the_same_for_16_bit_weights(bits, n, t):
         assert torch.equal(a[0].cpu(), -x.sign())
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [3000, 100000])
+@pytest.mark.parametrize("eps", [1e-17, 5.7e-11, 5.9e-11, 1e-8])
+def test_first_steps_of_16_bit_weights_on_both_sides_of_what_eps_hides(bits, n, eps):
+    """From 5.8e-11 (2^-39 / sqrt(1 - beta2)) an eps is so large that roots of squares below 2^-126 do not show next to it.
+    A weight is lr u rounded once to bf16 (half a step: 2^-8); the squares' loss is at most 3e-4 of the root."""
+    g = torch.Generator().manual_seed(n)
+    x = (10.0 ** (-19 + 2 * torch.rand(n, generator=g)) * (torch.randint(0, 2, (n,), generator=g) * 2 - 1)).to(BF16)
+    a = one(x, bits)
+    a = (*a[:2], *(s if s.dtype == torch.uint8 else s.float() for s in a[2:4]), *a[4:])
+    run(*a, lr=1.0, eps=eps)
+    w = x.double()
+    want = to.adamw(0 * w, w, 0 * w, 0 * w, 0.0, lr=1.0, betas=(0.9, 0.999), eps=eps, weight_decay=0.0)["p"]
+    off = (a[0].cpu().double() - want).abs() / want.abs()
+    assert float(off.max()) <= 2.0 ** -8 + 4e-4
+
+
 @pytest.mark.parametrize("n", [300, 40000])
 @pytest.mark.parametrize("bits", [32, 8])
 def test_weights_that_never_had_a_gradient_stay_without_eps(bits, n):
