@@ -356,7 +356,8 @@ int sv3d_layer_norm_forward(const sv3d_layer_norm_params *p, const void *x, cons
 
 /* Gradients of the call above; each of dx (contiguous, not dy's or x's memory), dweight, dbias may be NULL.  dweight and dbias
  * are sums over the rows in an order that the sizes fix; they need `workspace`, at least
- * sv3d_layer_norm_workspace() bytes, 16-byte aligned, whose content does not matter. */
+ * sv3d_layer_norm_workspace() bytes, 16-byte aligned, whose content does not matter: up to 4096 bytes for each column of rows of up
+ * to 8192 columns, up to 512 (8 for each row) beyond. */
 int sv3d_layer_norm_workspace(const sv3d_layer_norm_params *p, size_t *bytes);
 int sv3d_layer_norm_backward(const sv3d_layer_norm_params *p, const void *x, const void *dy, const void *weight,
                              const float *mean, const float *rstd, void *dx, void *dweight, void *dbias,

@@ -71,7 +71,9 @@ def add_training_flags(parser=None):
     p.add_argument('--print_scalars', type=int, default=1)
     p.add_argument('--seg_train', type=int, default=0)
     p.add_argument('--query_basis', type=int, default=0)
-    p.add_argument('--grad_clip', type=float, default=0.1)
+    p.add_argument('--grad_clip', type=float, default=0.1,
+                   help="largest norm of a network's gradients; 0 does not clip with --optim adamw and adamw8, and scales all "
+                        'gradients to nothing with adam')
     p.add_argument('--epoch_fraction', type=float, default=0.1)
     p.add_argument('--gc_freeze', type=int, default=1,
                    help='freeze the objects alive after set-up out of the garbage collector')
