@@ -641,7 +641,7 @@ def run_guarded(run, extras, out, rank, limit_s, poll_s=1.0):
     import threading
     import traceback
     lock = threading.Lock()
-    state = {"done": False}
+    state = {"done": False, "failed": None}
     store = _group_store()
     t_end = time.monotonic() + limit_s
 
@@ -662,7 +662,8 @@ def run_guarded(run, extras, out, rank, limit_s, poll_s=1.0):
             if store.check([FAILED_KEY]):
                 return store.get(FAILED_KEY).decode("utf-8", "replace")
         except Exception:                        # noqa: BLE001 - the store went away with its rank
-            return None
+            # rank 0 has read the key and left, or it died: there is nothing more to wait for
+            return state["failed"] or "rank 0, which holds the ranks' store, has left"
         return None
 
     def watch():
@@ -689,7 +690,7 @@ def run_guarded(run, extras, out, rank, limit_s, poll_s=1.0):
     except Exception as e:                       # noqa: BLE001 - reported in the line, the headline stands
         text = ("rank %d: %s: %s" % (rank, type(e).__name__, e))[:600]
         note("rank %d: an extra leg raised (%s):\n%s" % (rank, extras.get("_leg", "?"), traceback.format_exc()))
-        extras["extras_error"] = text
+        extras["extras_error"] = state["failed"] = text
         if store is not None:
             try:
                 store.set(FAILED_KEY, text)
